@@ -182,12 +182,12 @@ def _rope_freqs(case, theta=1e6, factor=8.0, original=4096, fast=32.0, slow=1.0)
 
 
 def _quantise(x, kv):
-    """Codes and scales of rows [..., d]: scale = absmax / largest code, code = x / scale to nearest even."""
-    most = _FP8_MAX if kv == "fp8" else _INT8_MAX
+    """Codes and scales of rows [..., d], M the largest code: scale = absmax / M, code = x * (M / absmax) to nearest
+    even."""
+    most = torch.full((), _FP8_MAX if kv == "fp8" else _INT8_MAX, device=x.device)
     x = x.float()
-    fine = torch.isfinite(x)
-    scale = torch.where(fine, x, torch.zeros_like(x)).abs().amax(-1) / torch.full((), most, device=x.device)
-    c = x / scale.unsqueeze(-1)
+    top = torch.where(torch.isfinite(x), x, torch.zeros_like(x)).abs().amax(-1)
+    scale, c = top / most, x * (most / top).unsqueeze(-1)
     c = torch.where(torch.isnan(c), torch.zeros_like(c), c).clamp(-most, most)
     return (c.to(torch.float8_e4m3fn) if kv == "fp8" else c.round().to(torch.int8)), scale
 
