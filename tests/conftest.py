@@ -16,12 +16,13 @@ for var in ("VSPEC_3BIT_RUNTIME_MODULE", "VSPEC_FUSED_BITS"):
     os.environ.pop(var, None)
 
 # The reference source tree (headers, Python modules) for the tests that read it:
-# VSPEC_REFERENCE, else the build environment's default from __graft_entry__.
+# VSPEC_REFERENCE, else the build environment's default from __graft_entry__ (a
+# path without the tree makes those tests skip; an empty one would make them
+# look under the working folder).
 if not os.environ.get("VSPEC_REFERENCE"):
     sys.path.insert(0, ROOT)
-    from __graft_entry__ import reference_tree  # noqa: E402
-    if reference_tree():
-        os.environ["VSPEC_REFERENCE"] = reference_tree()
+    from __graft_entry__ import REFERENCE_DEFAULT  # noqa: E402
+    os.environ["VSPEC_REFERENCE"] = REFERENCE_DEFAULT
 
 
 def pytest_configure(config):
