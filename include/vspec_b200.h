@@ -311,6 +311,172 @@ int vspec_b200_paged_gather(const void* d_k_pages, const void* d_v_pages, const 
                             size_t page_tokens, size_t num_kv_heads, size_t head_dim, int kv_dtype, void* d_k_out,
                             void* d_v_out, void* stream);
 
+/* ------------------------------------------------------------------------
+ * Speculative verification: the operators of a step that checks a tree of
+ * drafted tokens per sequence at once (no reference counterpart: its draft /
+ * verify control plane calls the single-token kernels).  Element types of
+ * activations and logits: fp32, fp16 or bf16; sums, softmax statistics and
+ * angles are held in 32 bits, results are rounded once.
+ * ------------------------------------------------------------------------ */
+#define VSPEC_B200_T_F32 0
+#define VSPEC_B200_T_F16 1
+#define VSPEC_B200_T_BF16 2
+
+/* Rotary positions.  For token t and pair i < rot_dim/2 of every head
+ *   (a, b) -> (a cos - b sin, a sin + b cos) * attn_factor,  angle = pos[t] * f_i,
+ * on the pairs (i, i + rot_dim/2), or (2i, 2i+1) with VSPEC_B200_ROPE_INTERLEAVED;
+ * dims from rot_dim on are copied (rot_dim <= head_dim <= 512, both even).  d_turns holds f_i / (2 pi) as a 64-bit
+ * fraction of a turn (vspec_b200_rope_turns): pos * turns mod 2^64 is the exact
+ * place in the turn, so angles keep their precision at any position.
+ * VSPEC_B200_ROPE_INVERSE rotates by -angle: the gradient of the call without
+ * it.  Rows are [tokens] x [heads][head_dim] with a token stride in elements
+ * (0 = heads * head_dim), e.g. slices of a fused q/k/v projection.  An output
+ * is either its input (same pointer and stride) or does not overlap any input;
+ * d_k may be NULL. */
+#define VSPEC_B200_ROPE_INTERLEAVED 0x1
+#define VSPEC_B200_ROPE_INVERSE 0x2
+typedef struct VspecB200RopeArgs {
+    const void* d_q;
+    const void* d_k;              /* NULL: q only */
+    void* d_q_out;
+    void* d_k_out;
+    const int32_t* d_pos;         /* [tokens] */
+    const uint64_t* d_turns;      /* [rot_dim/2] */
+    size_t tokens, num_q_heads, num_k_heads, head_dim, rot_dim;
+    size_t q_stride, k_stride, q_out_stride, k_out_stride;
+    float attn_factor;
+    int dtype;                    /* VSPEC_B200_T_* */
+    int flags;                    /* VSPEC_B200_ROPE_* */
+} VspecB200RopeArgs;
+int vspec_b200_rope(const VspecB200RopeArgs* args, void* stream);
+
+/* Host: fills turns[rot_dim/2] and *attn_factor for f_i = theta^(-2i/rot_dim),
+ *   PLAIN   as is;
+ *   LINEAR  f_i / factor (positions interpolated);
+ *   NTK     theta * factor^(rot_dim/(rot_dim-2)) in theta's place;
+ *   YARN    f_i below, f_i / factor above a linear ramp between the pairs that
+ *           turn beta_fast and beta_slow times in original_ctx positions, and
+ *           attn_factor = 0.1 ln(factor) + 1 (1 otherwise). */
+#define VSPEC_B200_ROPE_PLAIN 0
+#define VSPEC_B200_ROPE_LINEAR 1
+#define VSPEC_B200_ROPE_NTK 2
+#define VSPEC_B200_ROPE_YARN 3
+int vspec_b200_rope_turns(size_t rot_dim, double theta, int scaling, double factor, double original_ctx,
+                          double beta_fast, double beta_slow, uint64_t* turns, float* attn_factor);
+
+/* 8-bit KV pages: codes [num_pages][page_tokens][num_kv_heads][head_dim] bytes,
+ * e4m3 (KV_FP8) or two's complement (KV_INT8), and one fp32 scale per row
+ * [num_pages][page_tokens][num_kv_heads].  A row x of head_dim values:
+ *   scale = absmax / M,  code = round_to_even(x * (M / absmax)),  M = 448 or 127,
+ * absmax over its finite values; NaN is stored as 0, an infinity as +-M, a row
+ * of zeros has scale 0. */
+#define VSPEC_B200_KV_FP8 3
+#define VSPEC_B200_KV_INT8 4
+typedef struct VspecB200KvQuantArgs {
+    const void* d_k;              /* [rows] x [num_kv_heads][head_dim], src_dtype */
+    const void* d_v;
+    const int32_t* d_slots;       /* [rows] pool row page * page_tokens + slot, negative = row skipped; NULL = r */
+    size_t rows, num_kv_heads, head_dim;
+    size_t k_stride, v_stride;    /* elements between rows; 0 = num_kv_heads * head_dim */
+    size_t pool_rows;             /* num_pages * page_tokens */
+    void* d_k_codes;
+    void* d_v_codes;
+    float* d_k_scales;
+    float* d_v_scales;
+    int src_dtype;                /* VSPEC_B200_T_* */
+    int kv_dtype;                 /* VSPEC_B200_KV_FP8 or _INT8 */
+} VspecB200KvQuantArgs;
+/* Writes rows into the pools.  A slot at or past pool_rows is skipped and
+ * reported by vspec_b200_paged_attention_page_fault(); two rows with one slot
+ * leave either.  head_dim <= 512. */
+int vspec_b200_kv_quant_append(const VspecB200KvQuantArgs* args, void* stream);
+
+typedef struct VspecB200KvGatherArgs {
+    const void* d_k_codes;
+    const void* d_v_codes;
+    const float* d_k_scales;
+    const float* d_v_scales;
+    const int32_t* d_page_table;  /* [batch][max_pages_per_seq] */
+    const int32_t* d_cu_tokens;   /* [batch + 1] first output row of each sequence; the last entry <= total_tokens */
+    size_t batch, total_tokens, num_kv_heads, head_dim, page_tokens, max_pages_per_seq, num_pages;
+    void* d_k_out;                /* [total_tokens][num_kv_heads][head_dim], out_dtype */
+    void* d_v_out;
+    int out_dtype;                /* VSPEC_B200_T_* */
+    int kv_dtype;                 /* VSPEC_B200_KV_FP8 or _INT8 */
+} VspecB200KvGatherArgs;
+/* Reads the first cu[b+1] - cu[b] tokens of every sequence back, code * scale
+ * rounded once.  Bad page ids as in vspec_b200_paged_attention. */
+int vspec_b200_kv_quant_gather(const VspecB200KvGatherArgs* args, void* stream);
+
+/*
+ * Attention of a tree of drafted tokens over a paged cache.  Sequence b has
+ * ctx_len[b] committed tokens and cu_q[b+1] - cu_q[b] <= max_q drafted ones,
+ * whose K/V rows are in its pages at positions ctx_len[b] + j.  Drafted token i
+ * sees every committed token, and drafted token j where bit j of its mask row
+ * (bit j % 32 of word j / 32) is set:
+ *   out[i][h] = softmax_j(q[i][h] . K_j * scale) V_j,  kv head = h / (Hq/Hkv).
+ * d_mask NULL: j <= i (a chain, or a chunk of a prompt).  A row that sees
+ * nothing yields zeros; what a row does not see does not reach it, infinities
+ * and NaN included.  Pages as in vspec_b200_paged_attention (fp16), or 8-bit
+ * codes with scales as above.  max_q 1 is plain decode.  head_dim <= 256, a
+ * multiple of 8 (fp16 pages) or 16 (8-bit); pages, scales, q and out 16-byte
+ * aligned, q_stride a multiple of 8.
+ */
+typedef struct VspecB200TreeAttnArgs {
+    const void* d_q;              /* [total_q] x [num_q_heads][head_dim], q_dtype */
+    const void* d_k_pages;
+    const void* d_v_pages;
+    const float* d_k_scales;      /* 8-bit pages only */
+    const float* d_v_scales;
+    const int32_t* d_page_table;  /* [batch][max_pages_per_seq] */
+    const int32_t* d_ctx_len;     /* [batch] committed tokens */
+    const int32_t* d_cu_q;        /* [batch + 1] first row of each sequence; NULL = b * max_q */
+    const uint32_t* d_mask;       /* [total_q][mask_words], or NULL */
+    void* d_out;                  /* [total_q][num_q_heads][head_dim], q_dtype */
+    size_t batch, total_q, max_q, num_q_heads, num_kv_heads, head_dim;
+    size_t page_tokens, max_pages_per_seq, num_pages;
+    size_t max_ctx;               /* host-side upper bound of ctx_len + drafted; 0 = the page table's capacity */
+    size_t mask_words;            /* >= ceil(max_q / 32) */
+    size_t q_stride;              /* elements between rows of q; 0 = num_q_heads * head_dim */
+    float scale;
+    int q_dtype;                  /* VSPEC_B200_T_* */
+    int kv_dtype;                 /* VSPEC_B200_KV_F16, _FP8 or _INT8 */
+    void* d_workspace;            /* NULL = library-managed device scratch, grown on first use of a shape */
+    size_t workspace_bytes;
+} VspecB200TreeAttnArgs;
+size_t vspec_b200_tree_attention_workspace_bytes(size_t batch, size_t total_q, size_t max_q, size_t num_q_heads,
+                                                 size_t num_kv_heads, size_t head_dim, size_t max_ctx);
+int vspec_b200_tree_attention(const VspecB200TreeAttnArgs* args, void* stream);
+
+/*
+ * Log probabilities from logits, p = softmax(x * inv_temperature) over the
+ * allowed tokens of each row:
+ *   token_logprobs[r][g] = log p[tokens[r][g]]   (-inf for an id outside the vocabulary or not allowed)
+ *   entropy[r] = -sum p log p
+ *   top_ids / top_logprobs[r][0..top_k)  the allowed tokens of largest logit, ties to the lowest id
+ * A logit of -inf is not allowed; places past the allowed tokens hold id -1 and
+ * -inf.  A row with no allowed token has entropy 0.  NaN or +inf in an allowed
+ * place make the row's probabilities NaN (the top ids skip NaN); values in
+ * places that are not allowed are never used.  top_k <= 32.
+ */
+typedef struct VspecB200LogprobsArgs {
+    const void* d_logits;         /* [rows] x [vocab], dtype */
+    const uint32_t* d_allowed;    /* [rows][ceil(vocab/32)] bits, or NULL = all */
+    const int32_t* d_tokens;      /* [rows][num_tokens], or NULL */
+    float* d_token_logprobs;      /* [rows][num_tokens] */
+    float* d_entropy;             /* [rows], or NULL */
+    float* d_top_logprobs;        /* [rows][top_k], with top_k > 0 */
+    int32_t* d_top_ids;
+    size_t rows, vocab, row_stride;   /* row_stride in elements; 0 = vocab */
+    size_t num_tokens, top_k;
+    float inv_temperature;        /* at least 1e-30 */
+    int dtype;                    /* VSPEC_B200_T_* */
+    void* d_workspace;            /* NULL = library-managed device scratch, grown on first use of a shape */
+    size_t workspace_bytes;
+} VspecB200LogprobsArgs;
+size_t vspec_b200_logprobs_workspace_bytes(size_t rows, size_t vocab, size_t top_k);
+int vspec_b200_logprobs(const VspecB200LogprobsArgs* args, void* stream);
+
 /* ------------------------------------------------------ fp32 helpers */
 /* y = x / sqrt(mean(x^2) + eps) * w per row (src/kernel/cuda/cuda_rmsnorm_f32.cu:9-36). */
 int vspec_b200_rmsnorm_f32(const float* d_x, const float* d_w, float eps, size_t rows, size_t dim, float* d_y,

@@ -1096,6 +1096,18 @@ __global__ void paged_gather_kernel(const T* kp, const T* vp, const int32_t* tab
     }
 }
 
+int* attn_page_fault_device_ptr() {
+    static int* ptr[64] = {};
+    int dev = 0;
+    if (cudaGetDevice(&dev) != cudaSuccess || dev < 0 || dev >= 64) return nullptr;
+    if (!ptr[dev]) {
+        void* p = nullptr;
+        if (cudaGetSymbolAddress(&p, g_attn_page_fault) != cudaSuccess) return nullptr;
+        ptr[dev] = reinterpret_cast<int*>(p);
+    }
+    return ptr[dev];
+}
+
 int attn_read_and_clear_page_fault(int* out) {
     int v = 0, zero = 0;
     cudaError_t e = cudaMemcpyFromSymbol(&v, g_attn_page_fault, sizeof(int));

@@ -33,6 +33,8 @@ struct AttnParams {
 };
 
 int attn_read_and_clear_page_fault(int* out);
+// The flag's address on the current device, for the kernels of other files (NULL on error).
+int* attn_page_fault_device_ptr();
 
 int attn_choose_split(int batch, int hq, int hkv, int max_ctx, int page_tokens, int sms, int ctas_per_sm,
                       int max_staged_pages);

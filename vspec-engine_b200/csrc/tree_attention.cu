@@ -1,0 +1,191 @@
+// tree_attention.cu -- entry point of the tree attention: argument checks, the
+// plan (rows and context of a CTA) and the kernel that joins context pieces.
+#include "attention_kernels.cuh"
+#include "tree_attention_mma.cuh"
+
+#include <limits.h>
+#include <string.h>
+
+namespace vb200 {
+
+// One warp a (drafted token, head): out = sum_s O_s 2^(m_s - M) / sum_s l_s 2^(m_s - M), in piece order.
+__global__ void __launch_bounds__(256) tree_combine_kernel(const TreeParams p) {
+    pdl_wait();
+    pdl_trigger();
+    const int b = blockIdx.y;
+    int row0;
+    const int drafted = tree_rows(p, b, row0);
+    const long long r = (long long)blockIdx.x * 8 + (threadIdx.x >> 5);
+    const int lane = threadIdx.x & 31;
+    if (r >= (long long)drafted * p.hq) return;
+    const int total = max(p.ctx_len[b], 0) + drafted;
+    const int n = (total + p.split_tokens - 1) / p.split_tokens;
+    if (n <= 1) return;
+    const size_t row = (size_t)row0 * p.hq + (size_t)r;
+    const float* ml = p.part_ml + row * p.max_splits * 2;
+    float M = kTreeLowest;
+    for (int s = lane; s < n; s += 32) M = fmaxf(M, ml[2 * s]);
+    M = warp_max(M);
+    float L = 0.f;
+    for (int s = 0; s < n; ++s) L += ml[2 * s + 1] * tree_ex2(ml[2 * s] - M);
+    const float inv = L == 0.f ? 0.f : 1.0f / L;
+    for (int e = lane * 4; e < p.d; e += 128) {
+        float4 acc = {0.f, 0.f, 0.f, 0.f};
+        for (int s = 0; s < n; ++s) {
+            const float f = tree_ex2(ml[2 * s] - M);
+            const float4 v = *reinterpret_cast<const float4*>(p.part_o + (row * p.max_splits + s) * p.d + e);
+            acc.x += v.x * f; acc.y += v.y * f; acc.z += v.z * f; acc.w += v.w * f;
+        }
+        const size_t at = row * p.d + e;
+        tree_store(p.out, p.q_type, at, L == 0.f ? 0.f : acc.x * inv);
+        tree_store(p.out, p.q_type, at + 1, L == 0.f ? 0.f : acc.y * inv);
+        tree_store(p.out, p.q_type, at + 2, L == 0.f ? 0.f : acc.z * inv);
+        tree_store(p.out, p.q_type, at + 3, L == 0.f ? 0.f : acc.w * inv);
+    }
+}
+
+struct TreePlan {
+    int wr, row_tiles, split_tokens, max_splits;
+};
+
+// Rows a CTA: 16, 32 or 64, the fewest that hold a pair's rows.  Context
+// pieces: about four CTAs for each that is resident at once (sequences differ
+// in length), at least 128 tokens each.
+static TreePlan tree_plan(size_t batch, size_t max_q, size_t hq, size_t hkv, size_t max_ctx) {
+    TreePlan t;
+    const long long rows = (long long)max_q * (long long)(hq / hkv);
+    t.wr = rows <= 16 ? 1 : (rows <= 32 ? 2 : 4);
+    t.row_tiles = (int)((rows + 16 * t.wr - 1) / (16 * t.wr));
+    const long long pairs = (long long)batch * hkv * t.row_tiles;
+    const long long want = 4LL * 2 * device_sm_count();
+    const long long pieces = pairs >= want ? 1 : (want + pairs - 1) / pairs;
+    long long s = (((long long)max_ctx + pieces - 1) / pieces + kTreeTile - 1) / kTreeTile * kTreeTile;
+    if (s < 128) s = 128;
+    t.split_tokens = (int)s;
+    t.max_splits = (int)(((long long)max_ctx + s - 1) / s);
+    if (t.max_splits < 1) t.max_splits = 1;
+    return t;
+}
+
+static size_t tree_workspace(const TreePlan& t, size_t total_q, size_t hq, size_t d) {
+    return t.max_splits > 1 ? total_q * hq * (size_t)t.max_splits * (d + 2) * sizeof(float) : 0;
+}
+
+// Library-managed scratch, one grow-only buffer per device and host thread.
+struct TreeScratch {
+    void* ptr;
+    size_t cap;
+};
+static thread_local TreeScratch g_tree_scratch[64];
+
+static void* tree_scratch(size_t bytes) {
+    int dev = 0;
+    if (cudaGetDevice(&dev) != cudaSuccess || dev < 0 || dev >= 64) return nullptr;
+    TreeScratch& s = g_tree_scratch[dev];
+    if (s.cap < bytes) {
+        if (s.ptr) cudaFree(s.ptr);
+        s.ptr = nullptr;
+        s.cap = 0;
+        if (cudaMalloc(&s.ptr, bytes) != cudaSuccess) { s.ptr = nullptr; return nullptr; }
+        s.cap = bytes;
+    }
+    return s.ptr;
+}
+
+}  // namespace vb200
+
+using namespace vb200;
+
+extern "C" size_t vspec_b200_tree_attention_workspace_bytes(size_t batch, size_t total_q, size_t max_q, size_t hq,
+                                                            size_t hkv, size_t d, size_t max_ctx) {
+    if (batch == 0 || max_q == 0 || hq == 0 || hkv == 0 || hq % hkv != 0 || d == 0 || max_ctx == 0 ||
+        max_ctx > (size_t)INT_MAX || batch > 65535 || max_q > (size_t)INT_MAX / hq)
+        return 0;
+    return tree_workspace(tree_plan(batch, max_q, hq, hkv, max_ctx), total_q, hq, d);
+}
+
+extern "C" int vspec_b200_tree_attention(const VspecB200TreeAttnArgs* a, void* stream) {
+    if (!a) { set_error("args is NULL"); return VSPEC_B200_ERR_ARG; }
+    if (!elem_type_known(a->q_dtype)) { set_error("bad q_dtype %d", a->q_dtype); return VSPEC_B200_ERR_ARG; }
+    const bool f16 = a->kv_dtype == VSPEC_B200_KV_F16;
+    if (!f16 && a->kv_dtype != VSPEC_B200_KV_FP8 && a->kv_dtype != VSPEC_B200_KV_INT8) {
+        set_error("kv_dtype must be KV_F16, KV_FP8 or KV_INT8"); return VSPEC_B200_ERR_ARG;
+    }
+    if (!a->d_q || !a->d_k_pages || !a->d_v_pages || !a->d_page_table || !a->d_ctx_len || !a->d_out ||
+        (!f16 && (!a->d_k_scales || !a->d_v_scales))) {
+        set_error("NULL pointer argument"); return VSPEC_B200_ERR_ARG;
+    }
+    if (a->batch == 0 || a->max_q == 0 || a->num_q_heads == 0 || a->num_kv_heads == 0 || a->head_dim == 0 ||
+        a->page_tokens == 0 || a->max_pages_per_seq == 0 || a->num_pages == 0) {
+        set_error("zero dimension"); return VSPEC_B200_ERR_ARG;
+    }
+    if (a->num_q_heads % a->num_kv_heads != 0) { set_error("num_q_heads must be a multiple of num_kv_heads"); return VSPEC_B200_ERR_ARG; }
+    if (a->head_dim > 256 || a->head_dim % (f16 ? 8 : 16) != 0) {
+        set_error("head_dim must be a multiple of %d, at most 256", f16 ? 8 : 16); return VSPEC_B200_ERR_UNSUPPORTED;
+    }
+    const size_t lim = (size_t)INT_MAX;
+    if (a->batch > 65535 || a->num_q_heads > 65535 || a->max_q > lim / a->num_q_heads / 4 || a->total_q > lim ||
+        a->page_tokens > lim || a->num_pages > lim / a->page_tokens || a->max_pages_per_seq > lim) {
+        set_error("a size is too large"); return VSPEC_B200_ERR_ARG;
+    }
+    const size_t cap = a->max_pages_per_seq * a->page_tokens;
+    if (a->max_ctx > cap) { set_error("max_ctx %zu exceeds the page table capacity %zu", a->max_ctx, cap); return VSPEC_B200_ERR_ARG; }
+    const size_t max_ctx = a->max_ctx ? a->max_ctx : cap;
+    if (max_ctx > lim - 1024) { set_error("a size is too large"); return VSPEC_B200_ERR_ARG; }
+    if (a->d_mask && a->mask_words < (a->max_q + 31) / 32) { set_error("mask_words %zu is below ceil(max_q / 32)", a->mask_words); return VSPEC_B200_ERR_ARG; }
+    if (a->mask_words > lim) { set_error("a size is too large"); return VSPEC_B200_ERR_ARG; }
+    if (!a->d_cu_q && a->total_q != a->batch * a->max_q) { set_error("without d_cu_q total_q is batch * max_q"); return VSPEC_B200_ERR_ARG; }
+    const size_t qd = a->num_q_heads * a->head_dim;
+    if (a->q_stride && (a->q_stride < qd || a->q_stride % 8 != 0)) { set_error("q_stride must be a multiple of 8 and at least heads * head_dim"); return VSPEC_B200_ERR_ARG; }
+    const uintptr_t al = (uintptr_t)a->d_q | (uintptr_t)a->d_k_pages | (uintptr_t)a->d_v_pages | (uintptr_t)a->d_out |
+                         (f16 ? 0 : (uintptr_t)a->d_k_scales | (uintptr_t)a->d_v_scales);
+    if (al % 16 != 0) { set_error("q, out, pages and scales must be 16-byte aligned"); return VSPEC_B200_ERR_ARG; }
+    if (a->total_q == 0) return VSPEC_B200_OK;
+
+    const TreePlan plan = tree_plan(a->batch, a->max_q, a->num_q_heads, a->num_kv_heads, max_ctx);
+    TreeParams p;
+    memset(&p, 0, sizeof(p));
+    p.q = a->d_q;
+    p.k_pages = a->d_k_pages; p.v_pages = a->d_v_pages;
+    p.k_scales = a->d_k_scales; p.v_scales = a->d_v_scales;
+    p.table = a->d_page_table;
+    p.ctx_len = a->d_ctx_len;
+    p.cu_q = a->d_cu_q;
+    p.mask = a->d_mask;
+    p.out = a->d_out;
+    p.q_stride = a->q_stride ? a->q_stride : qd;
+    p.scale = a->scale;
+    p.batch = (int)a->batch; p.total_q = (int)a->total_q; p.max_q = (int)a->max_q;
+    p.hq = (int)a->num_q_heads; p.hkv = (int)a->num_kv_heads; p.group = p.hq / p.hkv; p.d = (int)a->head_dim;
+    p.page_tokens = (int)a->page_tokens; p.max_pages = (int)a->max_pages_per_seq; p.num_pages = (int)a->num_pages;
+    p.mask_words = (int)a->mask_words;
+    p.split_tokens = plan.split_tokens; p.max_splits = plan.max_splits; p.row_tiles = plan.row_tiles;
+    p.q_type = a->q_dtype;
+    if ((size_t)p.hkv * p.row_tiles > 65535) { set_error("a size is too large"); return VSPEC_B200_ERR_ARG; }
+    p.fault = attn_page_fault_device_ptr();
+    if (!p.fault) return cuda_status(cudaGetLastError(), "page fault flag");
+    const size_t need = tree_workspace(plan, a->total_q, a->num_q_heads, a->head_dim);
+    if (need) {
+        void* ws = a->d_workspace;
+        if (ws) {
+            if (a->workspace_bytes < need) { set_error("workspace too small (%zu < %zu)", a->workspace_bytes, need); return VSPEC_B200_ERR_ARG; }
+            if ((uintptr_t)ws % 16 != 0) { set_error("workspace must be 16-byte aligned"); return VSPEC_B200_ERR_ARG; }
+        } else {
+            ws = tree_scratch(need);
+            if (!ws) { set_error("cannot allocate %zu bytes of scratch", need); return VSPEC_B200_ERR_NOMEM; }
+        }
+        p.part_o = (float*)ws;
+        p.part_ml = p.part_o + a->total_q * a->num_q_heads * (size_t)p.max_splits * a->head_dim;
+    }
+    cudaStream_t st = (cudaStream_t)stream;
+    cudaError_t e = f16 ? tree_mma_launch<kTreeF16>(p, plan.wr, st)
+                  : a->kv_dtype == VSPEC_B200_KV_FP8 ? tree_mma_launch<kTreeFp8>(p, plan.wr, st)
+                                                     : tree_mma_launch<kTreeInt8>(p, plan.wr, st);
+    if (e != cudaSuccess) return cuda_status(e, "tree attention launch");
+    if (p.max_splits > 1) {
+        const size_t per = (size_t)p.max_q * p.hq;
+        e = launch_pdl(tree_combine_kernel, dim3((unsigned)((per + 7) / 8), p.batch), dim3(256), 0, st, p);
+        if (e != cudaSuccess) return cuda_status(e, "tree attention combine launch");
+    }
+    return VSPEC_B200_OK;
+}

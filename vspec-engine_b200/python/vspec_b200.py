@@ -28,6 +28,11 @@ F_SWIGLU = 0x10
 KV_F32 = 0
 KV_F16 = 1
 KV_INT3 = 2
+KV_FP8 = 3
+KV_INT8 = 4
+T_F32, T_F16, T_BF16 = 0, 1, 2
+ROPE_INTERLEAVED, ROPE_INVERSE = 0x1, 0x2
+ROPE_PLAIN, ROPE_LINEAR, ROPE_NTK, ROPE_YARN = 0, 1, 2, 3
 PATH_AUTO, PATH_GENERIC, PATH_WARPMMA, PATH_TCGEN05, PATH_RING, PATH_ROWS = 0, 1, 2, 3, 4, 5
 
 
@@ -78,6 +83,56 @@ class PagedAttnArgs(ctypes.Structure):
         ("batch", c_size_t), ("num_q_heads", c_size_t), ("num_kv_heads", c_size_t), ("head_dim", c_size_t),
         ("page_tokens", c_size_t), ("max_pages_per_seq", c_size_t), ("num_pages", c_size_t), ("max_ctx", c_size_t),
         ("scale", c_float), ("kv_dtype", c_int), ("d_workspace", c_void_p), ("workspace_bytes", c_size_t),
+    ]
+
+
+class RopeArgs(ctypes.Structure):
+    _fields_ = [
+        ("d_q", c_void_p), ("d_k", c_void_p), ("d_q_out", c_void_p), ("d_k_out", c_void_p), ("d_pos", c_void_p),
+        ("d_turns", c_void_p), ("tokens", c_size_t), ("num_q_heads", c_size_t), ("num_k_heads", c_size_t),
+        ("head_dim", c_size_t), ("rot_dim", c_size_t), ("q_stride", c_size_t), ("k_stride", c_size_t),
+        ("q_out_stride", c_size_t), ("k_out_stride", c_size_t), ("attn_factor", c_float), ("dtype", c_int),
+        ("flags", c_int),
+    ]
+
+
+class KvQuantArgs(ctypes.Structure):
+    _fields_ = [
+        ("d_k", c_void_p), ("d_v", c_void_p), ("d_slots", c_void_p), ("rows", c_size_t), ("num_kv_heads", c_size_t),
+        ("head_dim", c_size_t), ("k_stride", c_size_t), ("v_stride", c_size_t), ("pool_rows", c_size_t),
+        ("d_k_codes", c_void_p), ("d_v_codes", c_void_p), ("d_k_scales", c_void_p), ("d_v_scales", c_void_p),
+        ("src_dtype", c_int), ("kv_dtype", c_int),
+    ]
+
+
+class KvGatherArgs(ctypes.Structure):
+    _fields_ = [
+        ("d_k_codes", c_void_p), ("d_v_codes", c_void_p), ("d_k_scales", c_void_p), ("d_v_scales", c_void_p),
+        ("d_page_table", c_void_p), ("d_cu_tokens", c_void_p), ("batch", c_size_t), ("total_tokens", c_size_t),
+        ("num_kv_heads", c_size_t), ("head_dim", c_size_t), ("page_tokens", c_size_t),
+        ("max_pages_per_seq", c_size_t), ("num_pages", c_size_t), ("d_k_out", c_void_p), ("d_v_out", c_void_p),
+        ("out_dtype", c_int), ("kv_dtype", c_int),
+    ]
+
+
+class TreeAttnArgs(ctypes.Structure):
+    _fields_ = [
+        ("d_q", c_void_p), ("d_k_pages", c_void_p), ("d_v_pages", c_void_p), ("d_k_scales", c_void_p),
+        ("d_v_scales", c_void_p), ("d_page_table", c_void_p), ("d_ctx_len", c_void_p), ("d_cu_q", c_void_p),
+        ("d_mask", c_void_p), ("d_out", c_void_p), ("batch", c_size_t), ("total_q", c_size_t), ("max_q", c_size_t),
+        ("num_q_heads", c_size_t), ("num_kv_heads", c_size_t), ("head_dim", c_size_t), ("page_tokens", c_size_t),
+        ("max_pages_per_seq", c_size_t), ("num_pages", c_size_t), ("max_ctx", c_size_t), ("mask_words", c_size_t),
+        ("q_stride", c_size_t), ("scale", c_float), ("q_dtype", c_int), ("kv_dtype", c_int),
+        ("d_workspace", c_void_p), ("workspace_bytes", c_size_t),
+    ]
+
+
+class LogprobsArgs(ctypes.Structure):
+    _fields_ = [
+        ("d_logits", c_void_p), ("d_allowed", c_void_p), ("d_tokens", c_void_p), ("d_token_logprobs", c_void_p),
+        ("d_entropy", c_void_p), ("d_top_logprobs", c_void_p), ("d_top_ids", c_void_p), ("rows", c_size_t),
+        ("vocab", c_size_t), ("row_stride", c_size_t), ("num_tokens", c_size_t), ("top_k", c_size_t),
+        ("inv_temperature", c_float), ("dtype", c_int), ("d_workspace", c_void_p), ("workspace_bytes", c_size_t),
     ]
 
 
@@ -150,6 +205,15 @@ _sigs = {
     "vspec_b200_paged_attention_int3": ([POINTER(PagedAttnArgs), c_void_p, c_void_p, c_size_t, c_void_p], c_int),
     "vspec_b200_paged_gather": ([c_void_p, c_void_p, c_void_p, c_size_t, c_size_t, c_size_t, c_size_t, c_int, c_void_p,
                                  c_void_p, c_void_p], c_int),
+    "vspec_b200_rope": ([POINTER(RopeArgs), c_void_p], c_int),
+    "vspec_b200_rope_turns": ([c_size_t, ctypes.c_double, c_int] + [ctypes.c_double] * 4 +
+                              [c_void_p, POINTER(c_float)], c_int),
+    "vspec_b200_kv_quant_append": ([POINTER(KvQuantArgs), c_void_p], c_int),
+    "vspec_b200_kv_quant_gather": ([POINTER(KvGatherArgs), c_void_p], c_int),
+    "vspec_b200_tree_attention_workspace_bytes": ([c_size_t] * 7, c_size_t),
+    "vspec_b200_tree_attention": ([POINTER(TreeAttnArgs), c_void_p], c_int),
+    "vspec_b200_logprobs_workspace_bytes": ([c_size_t] * 3, c_size_t),
+    "vspec_b200_logprobs": ([POINTER(LogprobsArgs), c_void_p], c_int),
     "vspec_b200_rmsnorm_f32": ([c_void_p, c_void_p, c_float, c_size_t, c_size_t, c_void_p, c_void_p], c_int),
     "vspec_b200_linear_f32": ([c_void_p, c_void_p, c_size_t, c_size_t, c_size_t, c_void_p, c_void_p], c_int),
     "vspec_b200_silu_f32": ([c_void_p, c_size_t, c_void_p], c_int),
@@ -307,6 +371,63 @@ def anf_hybrid_linear(x: int, w2: int, s2: int, w4: int | None, s4: int | None, 
                       stream: int = 0) -> None:
     check(lib.vspec_b200_anf_hybrid_linear(x, w2, s2, w4, s4, zp4, y, hot, hot_count, m, n, k, n_blocks_int4, stream),
           "vspec_b200_anf_hybrid_linear")
+
+
+def rope_turns(rot_dim: int, theta: float, scaling: int = ROPE_PLAIN, factor: float = 1.0, original_ctx: float = 4096,
+               beta_fast: float = 32.0, beta_slow: float = 1.0) -> tuple[np.ndarray, float]:
+    """The frequencies rope() takes, uint64 [rot_dim/2] (upload once), and the factor on cos and sin."""
+    turns, mult = np.zeros(max(rot_dim // 2, 1), dtype=np.uint64), c_float(0.0)
+    check(lib.vspec_b200_rope_turns(rot_dim, theta, scaling, factor, original_ctx, beta_fast, beta_slow,
+                                    turns.ctypes.data, ctypes.byref(mult)), "vspec_b200_rope_turns")
+    return turns, mult.value
+
+
+def rope(q: int, k: int | None, q_out: int, k_out: int | None, pos: int, turns: int, tokens: int, hq: int, hk: int,
+         head_dim: int, rot_dim: int, dtype: int = T_F32, interleaved: bool = False, inverse: bool = False,
+         attn_factor: float = 1.0, q_stride: int = 0, k_stride: int = 0, q_out_stride: int = 0, k_out_stride: int = 0,
+         stream: int = 0) -> None:
+    flags = (ROPE_INTERLEAVED if interleaved else 0) | (ROPE_INVERSE if inverse else 0)
+    a = RopeArgs(q, k, q_out, k_out, pos, turns, tokens, hq, hk, head_dim, rot_dim, q_stride, k_stride, q_out_stride,
+                 k_out_stride, attn_factor, dtype, flags)
+    check(lib.vspec_b200_rope(ctypes.byref(a), stream), "vspec_b200_rope")
+
+
+def kv_quant_append(k: int, v: int, slots: int | None, rows: int, heads: int, head_dim: int, pool_rows: int,
+                    kv_dtype: int, k_codes: int, v_codes: int, k_scales: int, v_scales: int, src_dtype: int = T_F32,
+                    k_stride: int = 0, v_stride: int = 0, stream: int = 0) -> None:
+    a = KvQuantArgs(k, v, slots, rows, heads, head_dim, k_stride, v_stride, pool_rows, k_codes, v_codes, k_scales,
+                    v_scales, src_dtype, kv_dtype)
+    check(lib.vspec_b200_kv_quant_append(ctypes.byref(a), stream), "vspec_b200_kv_quant_append")
+
+
+def kv_quant_gather(k_codes: int, v_codes: int, k_scales: int, v_scales: int, page_table: int, cu_tokens: int,
+                    batch: int, total_tokens: int, heads: int, head_dim: int, page_tokens: int, max_pages: int,
+                    num_pages: int, kv_dtype: int, k_out: int, v_out: int, out_dtype: int = T_F16,
+                    stream: int = 0) -> None:
+    a = KvGatherArgs(k_codes, v_codes, k_scales, v_scales, page_table, cu_tokens, batch, total_tokens, heads, head_dim,
+                     page_tokens, max_pages, num_pages, k_out, v_out, out_dtype, kv_dtype)
+    check(lib.vspec_b200_kv_quant_gather(ctypes.byref(a), stream), "vspec_b200_kv_quant_gather")
+
+
+def tree_attention(q: int, k_pages: int, v_pages: int, k_scales: int | None, v_scales: int | None, page_table: int,
+                   ctx_len: int, cu_q: int | None, mask: int | None, out: int, batch: int, total_q: int, max_q: int,
+                   hq: int, hkv: int, d: int, page_tokens: int, max_pages: int, num_pages: int, max_ctx: int,
+                   scale: float, q_dtype: int = T_F32, kv_dtype: int = KV_F16, mask_words: int = 0, q_stride: int = 0,
+                   workspace: int | None = None, workspace_bytes: int = 0, stream: int = 0) -> None:
+    a = TreeAttnArgs(q, k_pages, v_pages, k_scales, v_scales, page_table, ctx_len, cu_q, mask, out, batch, total_q,
+                     max_q, hq, hkv, d, page_tokens, max_pages, num_pages, max_ctx, mask_words, q_stride, scale,
+                     q_dtype, kv_dtype, workspace, workspace_bytes)
+    check(lib.vspec_b200_tree_attention(ctypes.byref(a), stream), "vspec_b200_tree_attention")
+
+
+def logprobs(logits: int, rows: int, vocab: int, dtype: int = T_F32, tokens: int | None = None, num_tokens: int = 0,
+             token_logprobs: int | None = None, entropy: int | None = None, top_k: int = 0,
+             top_logprobs: int | None = None, top_ids: int | None = None, allowed: int | None = None,
+             inv_temperature: float = 1.0, row_stride: int = 0, workspace: int | None = None,
+             workspace_bytes: int = 0, stream: int = 0) -> None:
+    a = LogprobsArgs(logits, allowed, tokens, token_logprobs, entropy, top_logprobs, top_ids, rows, vocab, row_stride,
+                     num_tokens, top_k, inv_temperature, dtype, workspace, workspace_bytes)
+    check(lib.vspec_b200_logprobs(ctypes.byref(a), stream), "vspec_b200_logprobs")
 
 
 def page_fault_flag() -> int:
