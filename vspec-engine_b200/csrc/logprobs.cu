@@ -4,12 +4,10 @@
 // With m the row's maximum, S = sum exp((x - m)/T) and U = sum exp((x - m)/T) (x - m):
 //   log p(v) = (x_v - m)/T - ln S,   entropy = ln S - U / (T S).
 // A thread keeps (m, S, U) of what it has read and rescales when its maximum
-// grows; lanes, warps and the CTAs of a row join with the same rule.  The list
-// of the best is kept by each warp, one 64-bit key a lane in order (ordered
-// bits of the logit, then the complement of the id, so that ties go to the
-// lowest id); a value enters it only when it passes the CTA's threshold, the
-// best k-th key that any of its warps holds, so after the first few thousand
-// values almost none do.
+// grows; lanes, warps and the CTAs of a row join with the same rule.  The best
+// are 64-bit keys (ordered bits of the logit, then the complement of the id, so
+// that ties go to the lowest id); only values that pass a threshold are looked
+// at again, which after a row's first block almost none do.
 // Bound by memory: a logit is read once.  Few rows: several CTAs share a row
 // and the last one to finish joins their parts in CTA order (no result depends
 // on the order of arrival).
@@ -23,6 +21,7 @@ namespace vb200 {
 constexpr int kLpThreads = 512;
 constexpr int kLpWarps = kLpThreads / 32;
 constexpr int kLpMaxTop = 32;
+constexpr int kLpCandidates = 2048;
 constexpr int kLpMaxSplitRows = 2048;              // rows above this are never split
 constexpr size_t kLpCounterBytes = kLpMaxSplitRows * sizeof(unsigned);
 constexpr float kLpLowest = -3.402823466e+38f;
@@ -84,182 +83,294 @@ __device__ __forceinline__ LpStats lp_join(const LpStats a, const LpStats b, flo
     return r;
 }
 
-// A warp's best keys, lane l holding the l-th largest.
-__device__ __forceinline__ void lp_insert(unsigned long long& best, unsigned long long key, int lane) {
-    const int at = __popc(__ballot_sync(0xffffffffu, best > key));
-    const unsigned long long up = __shfl_up_sync(0xffffffffu, best, 1);
-    best = lane < at ? best : (lane == at ? key : up);
+// Sorts 32 keys over a warp's lanes, the largest in lane 0.
+__device__ __forceinline__ unsigned long long lp_warp_sort(unsigned long long k, int lane) {
+#pragma unroll
+    for (int size = 2; size <= 32; size <<= 1)
+#pragma unroll
+        for (int o = size >> 1; o > 0; o >>= 1) {
+            const unsigned long long q = __shfl_xor_sync(0xffffffffu, k, o);
+            const bool larger = ((lane & o) == 0) == ((lane & size) == 0);   // this lane keeps the larger one
+            k = (q > k) == larger ? q : k;
+        }
+    return k;
 }
 
+struct LpShared {
+    unsigned long long lists[kLpWarps][32];   // the warps' sorted keys of a selection
+    unsigned long long top[kLpMaxTop];        // the best so far, in order
+    unsigned long long bound[kLpMaxTop];      // the best of the threads' maxima
+    unsigned long long cand[kLpCandidates];
+    LpStats stats[kLpWarps];
+    int count, last;
+};
+
+// The larger half of two ordered lists of 32, in order again: the pairs (i, 31 - i) leave a bitonic sequence.
+__device__ __forceinline__ unsigned long long lp_warp_merge(unsigned long long a, unsigned long long b_reversed, int lane) {
+    unsigned long long k = a > b_reversed ? a : b_reversed;
+#pragma unroll
+    for (int o = 16; o > 0; o >>= 1) {
+        const unsigned long long q = __shfl_xor_sync(0xffffffffu, k, o);
+        k = (q > k) == ((lane & o) == 0) ? q : k;
+    }
+    return k;
+}
+
+// out[0..32) = the largest of the CTA's keys (one a thread, 0 = none), in
+// order: every warp sorts its own, then the lists join in pairs.  Called by all
+// threads; 1 + log2(warps) barriers and one behind.
+__device__ __noinline__ void lp_select(LpShared& sm, unsigned long long key, unsigned long long* out) {
+    const int warp = threadIdx.x >> 5, lane = threadIdx.x & 31;
+    key = lp_warp_sort(key, lane);
+    sm.lists[warp][lane] = key;
+#pragma unroll 1
+    for (int n = kLpWarps / 2; n > 0; n >>= 1) {
+        __syncthreads();
+        if (warp < n) {
+            key = lp_warp_merge(key, sm.lists[warp + n][31 - lane], lane);
+            sm.lists[warp][lane] = key;
+        }
+    }
+    if (warp == 0) out[lane] = key;
+    __syncthreads();
+}
+
+// sm.top = the best of itself and n keys.
+template <typename Load>
+__device__ __forceinline__ void lp_take_keys(LpShared& sm, int n, Load load) {
+    constexpr int kFresh = kLpThreads - kLpMaxTop;
+    for (int at = 0; at < n; at += kFresh) {
+        const int i = at + (int)threadIdx.x - kLpMaxTop;
+        const unsigned long long key = threadIdx.x < kLpMaxTop ? sm.top[threadIdx.x] : (i < n ? load(i) : 0ull);
+        lp_select(sm, key, sm.top);
+    }
+}
+
+// Statistics of the CTA in every thread of warp 0 (one order of joining, whatever ran first).
+__device__ __forceinline__ LpStats lp_join_cta(LpShared& sm, LpStats st, float c) {
+    const int warp = threadIdx.x >> 5, lane = threadIdx.x & 31;
+    auto join_lanes = [&](int from) {
+        for (int o = from; o > 0; o >>= 1) {
+            LpStats q;
+            q.m = __shfl_xor_sync(0xffffffffu, st.m, o);
+            q.s = __shfl_xor_sync(0xffffffffu, st.s, o);
+            q.u = __shfl_xor_sync(0xffffffffu, st.u, o);
+            st = (lane & o) ? lp_join(q, st, c) : lp_join(st, q, c);
+        }
+    };
+    join_lanes(16);
+    __syncthreads();
+    if (lane == 0) sm.stats[warp] = st;
+    __syncthreads();
+    if (warp == 0) {
+        st = sm.stats[lane % kLpWarps];
+        join_lanes(kLpWarps / 2);
+    }
+    return st;
+}
+
+// A CTA walks over its part of a row in blocks of kLpThreads * U vectors, one
+// barrier a block, with the next block's loads in flight.  Values at or above
+// the threshold go to a candidate list; when more than 32 threads hold one (the
+// first block, rows that rise), the threshold is first raised to the top_k-th
+// largest of the threads' maxima, below which no value can be among the best.
+// At most 32 threads (top_k <= 32) then add their U * V values.
 template <typename T, int V, bool ALLOWED, bool TOP>
-__global__ void __launch_bounds__(kLpThreads) logprobs_kernel(const LpParams p) {
+__global__ void __launch_bounds__(kLpThreads, 2) logprobs_kernel(const LpParams p) {
     pdl_wait();
     pdl_trigger();
+    constexpr int U = 16 / V;   // vectors a thread and block (16 values: more spill)
+    static_assert(32 + 32 * U * V <= kLpCandidates, "candidate list");
     const size_t row = blockIdx.y;
-    const int tid = threadIdx.x, warp = tid >> 5, lane = tid & 31;
+    const int tid = threadIdx.x, lane = tid & 31;
     const T* x = (const T*)p.logits + row * p.row_stride;
     const uint32_t* bits = ALLOWED ? p.allowed + row * p.words : nullptr;
-    __shared__ unsigned long long sm_thr;
-    __shared__ unsigned long long sm_keys[kLpWarps][kLpMaxTop];
-    __shared__ LpStats sm_stats[kLpWarps];
-    __shared__ unsigned sm_last;
-    if (TOP && tid == 0) sm_thr = 0;
-    if (TOP) __syncthreads();
+    __shared__ LpShared sm;
+    if (TOP) {
+        if (tid < kLpMaxTop) sm.top[tid] = 0;
+        if (tid == 0) sm.count = 0;
+    }
 
     const float c = p.inv_t * 1.4426950408889634f;
     LpStats st = {kLpLowest, 0.f, 0.f};
-    unsigned long long best = 0, thr = 0;
+    unsigned long long thr = 0;   // the same in every thread
     float thr_v = -INFINITY;
-
-    // one vector of values starting at id j; n of them count
-    auto take = [&](const float (&v)[V], int j, int n) {
-        uint32_t ok = n >= V ? 0xffffffffu : (n > 0 ? (1u << n) - 1u : 0u);
-        if (ALLOWED && n > 0) {
-            uint32_t b = bits[j >> 5] >> (j & 31);
-            if ((j & 31) + (n < V ? n : V) > 32) b |= bits[(j >> 5) + 1] << (32 - (j & 31));
-            ok &= b;
-        }
-        float w[V], top = -INFINITY;
-#pragma unroll
-        for (int i = 0; i < V; ++i) {
-            w[i] = (ok >> i) & 1u ? v[i] : -INFINITY;
-            top = fmaxf(top, w[i]);
-        }
-        if (top > st.m) {
-            const float d = st.m - top, f = ex2_approx(d * c);
-            st.u = lp_rescale_u(st, d, f);
-            st.s *= f;
-            st.m = top;
-        }
-#pragma unroll
-        for (int i = 0; i < V; ++i) {
-            const float d = max_nan(w[i] - st.m, kLpLowest);   // -inf - m stays finite, so that 0 * d is 0
-            const float e = ex2_approx(d * c);
-            st.s += e;
-            st.u = fmaf(e, d, st.u);
-        }
-        if (TOP) {
-            if (__any_sync(0xffffffffu, top >= thr_v && top > -INFINITY)) {
-                const unsigned long long shared_thr = *(volatile unsigned long long*)&sm_thr;
-                if (shared_thr > thr) thr = shared_thr;
-                const unsigned long long before = thr;
-#pragma unroll
-                for (int i = 0; i < V; ++i) {
-                    // NaN fails the comparison; -inf has no place in the list
-                    const unsigned long long key = w[i] > -INFINITY ? lp_key(w[i], j + i) : 0ull;
-                    unsigned in = __ballot_sync(0xffffffffu, key > thr);
-                    while (in) {
-                        const int from = __ffs(in) - 1;
-                        in &= in - 1;
-                        const unsigned long long k = __shfl_sync(0xffffffffu, key, from);
-                        if (k > thr) {
-                            lp_insert(best, k, lane);
-                            const unsigned long long mine = __shfl_sync(0xffffffffu, best, p.top_k - 1);
-                            if (mine > thr) thr = mine;
-                        }
-                    }
-                }
-                if (lane == 0 && thr > before) atomicMax(&sm_thr, thr);
-                thr_v = thr ? lp_key_value(thr) : -INFINITY;
-            }
-        }
-    };
+    int pending = 32;   // the list holds no more candidates than this
+    // Draining raises the threshold to what all values so far allow; after 4, 16, ... blocks with candidates its cost
+    // (a selection, about two blocks' work) buys blocks in which fewer warps have any.
+    int offers = 0, next_drain = 4;
 
     const int j0 = blockIdx.x * p.chunk, j1 = min(p.vocab, j0 + p.chunk);
     // values before the first 16-byte boundary, whole vectors, values after the last
     const int off = (int)(((uintptr_t)(x + j0) % (V * sizeof(T))) / sizeof(T));
     const int head = off ? min(V - off, j1 - j0) : 0;
     const int vecs = j1 > j0 + head ? (j1 - j0 - head) / V : 0;
-    const int body = j0 + head;
-    constexpr int U = 4;   // vectors in flight a thread
+    const int body = j0 + head, tail = body + vecs * V;
     using W = Vec<T, V>;
-    for (int g0 = 0; g0 < vecs; g0 += kLpThreads * U) {
-        W w[U];
-#pragma unroll
-        for (int i = 0; i < U; ++i) {
-            const int g = g0 + i * kLpThreads + tid;
-            if (g < vecs) w[i] = *reinterpret_cast<const W*>(x + body + (size_t)g * V);
-        }
-#pragma unroll
-        for (int i = 0; i < U; ++i) {
-            const int g = g0 + i * kLpThreads + tid;
-            if (g0 + i * kLpThreads + warp * 32 >= vecs) break;   // the whole warp is past the end
-            float v[V];
-#pragma unroll
-            for (int e = 0; e < V; ++e) v[e] = g < vecs ? elem_to_f32<T>(w[i].e[e]) : 0.f;
-            take(v, body + g * V, g < vecs ? V : 0);
-        }
-    }
-    // the ends, a value a lane of warp 0: lanes 0-15 the head, 16-31 the tail
-    if (warp == 0) {
-        const int j = lane < 16 ? j0 + lane : body + vecs * V + lane - 16;
-        const bool in = lane < 16 ? lane < head : j < j1;
-        float v[V];
-#pragma unroll
-        for (int e = 0; e < V; ++e) v[e] = 0.f;
-        if (in) v[0] = elem_to_f32<T>(x[j]);
-        take(v, j, in ? 1 : 0);
-    }
 
-    // ---- join the warps ----
+    // value e of a vector, -inf where it is not allowed (a vector past the end is all -inf)
+    auto value = [&](const W& w, int e, uint32_t ok) {
+        const float v = elem_to_f32<T>(w.e[e]);
+        return !ALLOWED || ((ok >> e) & 1u) ? v : -INFINITY;
+    };
+    auto allowed_bits = [&](int j, int n) -> uint32_t {   // bits of ids j .. j + n - 1
+        uint32_t ok = (1u << n) - 1u;
+        if (ALLOWED) {
+            uint32_t b = bits[j >> 5] >> (j & 31);
+            if ((j & 31) + n > 32) b |= bits[(j >> 5) + 1] << (32 - (j & 31));
+            ok &= b;
+        }
+        return ok;
+    };
+    auto add = [&](float v) {
+        const float d = max_nan(v - st.m, kLpLowest);   // -inf - m stays finite, so that 0 * d is 0
+        const float e = ex2_approx(d * c);
+        st.s += e;
+        st.u = fmaf(e, d, st.u);
+    };
+    auto grow = [&](float top) {
+        if (top > st.m) {
+            const float d = st.m - top, f = ex2_approx(d * c);
+            st.u = lp_rescale_u(st, d, f);
+            st.s *= f;
+            st.m = top;
+        }
+    };
+    auto drain = [&]() {   // candidates into the list of the best
+        const int n = sm.count;
+        lp_take_keys(sm, n, [&](int i) { return sm.cand[i]; });
+        if (tid == 0) sm.count = 0;
+        __syncthreads();
+        const unsigned long long k = sm.top[p.top_k - 1];
+        if (k > thr) { thr = k; thr_v = lp_key_value(k); }
+    };
+    // candidates of a block: for_each(f, bound) calls f with the values and ids of this thread's vectors that reach
+    // the bound
+    auto offer = [&](float top, auto for_each) {
+        const int n = __syncthreads_count(top >= thr_v && top > -INFINITY);
+        if (n == 0) return;
+        // room for what this block may add, from a bound that every thread holds
+        const int most = (n > 32 ? 32 : n) * (U * V);
+        if (pending + most > kLpCandidates || ++offers == next_drain) {
+            drain();
+            pending = 0;
+            offers = 0;
+            next_drain *= 4;
+        }
+        pending += most;
+        if (n > 32) {
+            unsigned long long best = 0;
+            for_each([&](float v, int id) {
+                const unsigned long long k = v > -INFINITY ? lp_key(v, id) : 0ull;
+                best = k > best ? k : best;
+            }, -INFINITY);
+            lp_select(sm, best, sm.bound);
+            const unsigned long long k = sm.bound[p.top_k - 1];
+            if (k > thr) { thr = k; thr_v = lp_key_value(k); }
+        }
+        if (top >= thr_v)
+            for_each([&](float v, int id) {
+                // NaN fails the comparison; -inf has no place in the list
+                if (v >= thr_v && v > -INFINITY) {
+                    const unsigned long long k = lp_key(v, id);
+                    if (k >= thr) sm.cand[atomicAdd(&sm.count, 1)] = k;
+                }
+            }, thr_v);
+    };
+
+    W cur[U], nxt[U];
+    auto fetch = [&](int g0, W (&w)[U]) {
 #pragma unroll
-    for (int o = 16; o > 0; o >>= 1) {
-        LpStats q;
-        q.m = __shfl_xor_sync(0xffffffffu, st.m, o);
-        q.s = __shfl_xor_sync(0xffffffffu, st.s, o);
-        q.u = __shfl_xor_sync(0xffffffffu, st.u, o);
-        // one order for both lanes of a pair
-        st = (lane & o) ? lp_join(q, st, c) : lp_join(st, q, c);
-    }
-    if (lane == 0) sm_stats[warp] = st;
-    if (TOP) sm_keys[warp][lane] = lane < p.top_k ? best : 0ull;
-    __syncthreads();
-    if (warp != 0) return;
-    st = sm_stats[0];
-    for (int w = 1; w < kLpWarps; ++w) st = lp_join(st, sm_stats[w], c);
-    if (TOP) {
-        for (int w = 1; w < kLpWarps; ++w) {
-            for (int i = 0; i < p.top_k; ++i) {
-                const unsigned long long k = sm_keys[w][i];
-                if (k <= __shfl_sync(0xffffffffu, best, p.top_k - 1)) break;   // the rest are smaller
-                lp_insert(best, k, lane);
+        for (int i = 0; i < U; ++i) {
+            const int g = g0 + i * kLpThreads + tid;
+            if (g < vecs) {
+                w[i] = *reinterpret_cast<const W*>(x + body + (size_t)g * V);
+            } else {
+#pragma unroll
+                for (int e = 0; e < V; ++e) w[i].e[e] = elem_from_f32<T>(-INFINITY);
             }
         }
+    };
+    fetch(0, cur);
+    // the ends, a value a thread: threads 0-15 the head, 16-31 the tail
+    {
+        const int j = tid < 16 ? j0 + tid : tail + tid - 16;
+        const bool in = tid < 16 ? tid < head : tid < 32 && j < j1;
+        float v = -INFINITY;
+        if (in && (allowed_bits(j, 1) & 1u)) v = elem_to_f32<T>(x[j]);
+        grow(v);
+        add(v);
+        if (TOP) {
+            __syncthreads();
+            // at most 30 candidates; the threshold is still open
+            if (v > -INFINITY) sm.cand[atomicAdd(&sm.count, 1)] = lp_key(v, j);
+        }
     }
+    for (int g0 = 0; g0 < vecs; g0 += kLpThreads * U) {
+        fetch(g0 + kLpThreads * U, nxt);
+        uint32_t ok[U];
+        float top = -INFINITY, vec_top[U];
+#pragma unroll
+        for (int i = 0; i < U; ++i) {
+            const int g = g0 + i * kLpThreads + tid;
+            ok[i] = ALLOWED && g < vecs ? allowed_bits(body + g * V, V) : 0u;
+            vec_top[i] = -INFINITY;
+#pragma unroll
+            for (int e = 0; e < V; ++e) vec_top[i] = fmaxf(vec_top[i], value(cur[i], e, ok[i]));
+            top = fmaxf(top, vec_top[i]);
+        }
+        grow(top);
+#pragma unroll
+        for (int i = 0; i < U; ++i)
+#pragma unroll
+            for (int e = 0; e < V; ++e) add(value(cur[i], e, ok[i]));
+        if (TOP)
+            offer(top, [&](auto f, float bound) {
+#pragma unroll
+                for (int i = 0; i < U; ++i) {
+                    if (vec_top[i] < bound) continue;
+#pragma unroll
+                    for (int e = 0; e < V; ++e)
+                        f(value(cur[i], e, ok[i]), body + (g0 + i * kLpThreads + tid) * V + e);
+                }
+            });
+#pragma unroll
+        for (int i = 0; i < U; ++i) cur[i] = nxt[i];
+    }
+
+    st = lp_join_cta(sm, st, c);   // its barriers close the candidate list
+    if (TOP) drain();
 
     if (p.splits > 1) {
         const size_t at = row * p.splits + blockIdx.x;
-        if (TOP && lane < p.top_k) p.part_keys[at * p.top_k + lane] = best;
-        if (lane == 0) {
+        if (TOP && tid < p.top_k) p.part_keys[at * p.top_k + tid] = sm.top[tid];
+        if (tid == 0) {
             p.part_stats[at * 4 + 0] = st.m;
             p.part_stats[at * 4 + 1] = st.s;
             p.part_stats[at * 4 + 2] = st.u;
         }
         __threadfence();
-        __syncwarp();
-        if (lane == 0) {
-            sm_last = atomicAdd(&p.counters[row], 1u) == (unsigned)p.splits - 1;
-            if (sm_last) p.counters[row] = 0;
+        __syncthreads();
+        if (tid == 0) {
+            sm.last = atomicAdd(&p.counters[row], 1u) == (unsigned)p.splits - 1;
+            if (sm.last) p.counters[row] = 0;
         }
-        __syncwarp();
-        if (!sm_last) return;
+        __syncthreads();
+        if (!sm.last) return;
         __threadfence();
-        const volatile float* ps = p.part_stats + row * p.splits * 4;
-        const volatile unsigned long long* pk = p.part_keys + row * p.splits * (size_t)p.top_k;
-        st = {ps[0], ps[1], ps[2]};
-        if (TOP) best = lane < p.top_k ? pk[lane] : 0ull;
-        for (int i = 1; i < p.splits; ++i) {
-            st = lp_join(st, LpStats{ps[i * 4], ps[i * 4 + 1], ps[i * 4 + 2]}, c);
-            if (TOP) {
-                const unsigned long long mine = lane < p.top_k ? pk[(size_t)i * p.top_k + lane] : 0ull;
-                for (int e = 0; e < p.top_k; ++e) {
-                    const unsigned long long k = __shfl_sync(0xffffffffu, mine, e);
-                    if (k <= __shfl_sync(0xffffffffu, best, p.top_k - 1)) break;
-                    lp_insert(best, k, lane);
-                }
-            }
+        st = {kLpLowest, 0.f, 0.f};
+        const float* ps = p.part_stats + row * p.splits * 4;
+        for (int i = tid; i < p.splits; i += kLpThreads)
+            st = lp_join(st, LpStats{__ldcg(ps + i * 4), __ldcg(ps + i * 4 + 1), __ldcg(ps + i * 4 + 2)}, c);
+        st = lp_join_cta(sm, st, c);
+        if (TOP) {
+            const unsigned long long* pk = p.part_keys + row * p.splits * (size_t)p.top_k;
+            if (tid < kLpMaxTop) sm.top[tid] = 0;
+            __syncthreads();
+            lp_take_keys(sm, p.splits * p.top_k, [&](int i) { return __ldcg(pk + i); });
         }
     }
+    if (tid >= 32) return;
 
     // ---- results ----
     const bool none = st.s == 0.f;
@@ -267,6 +378,7 @@ __global__ void __launch_bounds__(kLpThreads) logprobs_kernel(const LpParams p) 
     if (lane == 0 && p.entropy) p.entropy[row] = none ? 0.f : ln_s - st.u * p.inv_t / st.s;
     if (TOP && lane < p.top_k) {
         const size_t at = row * p.top_k + lane;
+        const unsigned long long best = sm.top[lane];
         p.top_ids[at] = best ? lp_key_id(best) : -1;
         p.top_lp[at] = best ? (lp_key_value(best) - st.m) * p.inv_t - ln_s : -INFINITY;
     }
@@ -281,10 +393,12 @@ __global__ void __launch_bounds__(kLpThreads) logprobs_kernel(const LpParams p) 
     }
 }
 
-// CTAs a row: enough for about four on every SM together, each with at least 4096 values.
+// CTAs a row: what fills the two resident on every SM, each with at least 4096
+// values. A row's fixed cost (two selections) is why rows that fill the SMs
+// are not split for a better balance.
 static int lp_splits(size_t rows, size_t vocab) {
     if (rows >= (size_t)kLpMaxSplitRows) return 1;
-    size_t s = (4 * (size_t)device_sm_count() + rows - 1) / rows;
+    size_t s = 2 * (size_t)device_sm_count() / rows;
     const size_t most = vocab / 4096;
     if (s > most) s = most;
     return s < 1 ? 1 : (int)s;

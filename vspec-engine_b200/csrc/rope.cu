@@ -9,15 +9,22 @@
 // bits, as a signed fraction of a half turn, go to sincospif, which then needs
 // no range reduction and holds 24 bits at any position.
 //
-// Memory-bound: every value is read and written once.  One CTA works on the
-// heads of one token; a thread keeps the sines of its pairs and walks over
-// heads, so a sincospif serves all heads that the thread visits.
+// Memory-bound: every value is read and written once.  A CTA works on up to
+// four tokens: its threads share out the tokens' angles (one sincospif a pair
+// and token, kept in shared memory) while the first rows are on their way, then
+// every thread walks over the heads of each token with a fixed place in the
+// head.  Without the sharing, 16 threads with the same place computed the same
+// sines and those took longer than the rows (75 us against DRAM's 26 us at 8192
+// tokens of 32 + 8 heads of 128 in bf16).
 #include "elem_types.cuh"
 
 #include <math.h>
 #include <string.h>
 
 namespace vb200 {
+
+constexpr int kRopeThreads = 256;
+constexpr int kRopePairs = 256;   // angles of a token group
 
 struct RopeParams {
     const void *q, *k;
@@ -27,61 +34,94 @@ struct RopeParams {
     size_t q_stride, k_stride, q_out_stride, k_out_stride;
     int hq, heads, d, rot;     // heads = hq + hk
     int units, rot_units;      // units of 2V elements a head (the rotated ones first)
+    int group;                 // tokens a CTA
+    size_t tokens;
     float mult, sign;          // attn_factor; -1 for the inverse rotation
 };
 
-// Grid (tokens, head slices).  A unit is 2V elements: V pairs (for halves, V
-// elements at i and V at i + rot/2; interleaved, 2V in a row), or 2V elements
-// of the copied tail.
+// Grid (token groups, head slices).  A unit is 2V elements: V pairs (for
+// halves, V elements at i and V at i + rot/2; interleaved, 2V in a row), or 2V
+// elements of the copied tail.
 template <typename T, int V, bool INTER>
-__global__ void __launch_bounds__(256) rope_kernel(const RopeParams p) {
+__global__ void __launch_bounds__(kRopeThreads, 4) rope_kernel(const RopeParams p) {
     pdl_wait();
     pdl_trigger();
-    const size_t t = blockIdx.x;
+    __shared__ __align__(16) float sm_cos[kRopePairs], sm_sin[kRopePairs];   // [token of the group][pair]
+    const int pairs = p.rot / 2, per = kRopeThreads / p.units;
+    const size_t t0 = (size_t)blockIdx.x * p.group;
+    const int tokens = (int)min((size_t)p.group, p.tokens - t0);
     const int u = threadIdx.x % p.units;
-    const int step = (int)(blockDim.x / p.units) * gridDim.y;
-    int h = (int)(threadIdx.x / p.units) + (int)(blockDim.x / p.units) * blockIdx.y;
-    if (threadIdx.x >= (blockDim.x / p.units) * p.units) return;
+    const int step = per * gridDim.y, w0 = (int)threadIdx.x / p.units + per * blockIdx.y;
     const bool turn = u < p.rot_units;
     const int i0 = INTER || !turn ? 2 * V * u : V * u;                    // first element of the unit
-    const int i1 = INTER || !turn ? i0 + V : i0 + p.rot / 2;              // its second vector
-    float cs[V], sn[V];
-    if (turn) {
-        const uint64_t pos = (uint64_t)(int64_t)p.pos[t];
-#pragma unroll
-        for (int j = 0; j < V; ++j) {
-            const int32_t part = (int32_t)((pos * p.turns[V * u + j]) >> 32);
-            sincospif((float)part * (1.0f / 2147483648.0f), &sn[j], &cs[j]);
-            sn[j] *= p.sign * p.mult;
-            cs[j] *= p.mult;
-        }
-    }
+    const int i1 = INTER || !turn ? i0 + V : i0 + pairs;                  // its second vector
+    const int rows = (int)threadIdx.x < per * p.units ? tokens * p.heads : 0;   // (token, head) rows to walk over
     using W = Vec<T, V>;
-    for (; h < p.heads; h += step) {
-        const bool is_q = h < p.hq;
-        const T* src = is_q ? (const T*)p.q + t * p.q_stride + (size_t)h * p.d
-                            : (const T*)p.k + t * p.k_stride + (size_t)(h - p.hq) * p.d;
-        T* dst = is_q ? (T*)p.q_out + t * p.q_out_stride + (size_t)h * p.d
-                      : (T*)p.k_out + t * p.k_out_stride + (size_t)(h - p.hq) * p.d;
-        if (!turn && src == dst) continue;
-        W a = *reinterpret_cast<const W*>(src + i0), b = *reinterpret_cast<const W*>(src + i1);
-        if (turn) {
-            T v[2 * V];
+    constexpr int H = 2;   // rows with loads in flight
+    W a[H], b[H];
+    T* dst[H];
+    int at[H];             // first angle of the row's token
+    auto fetch = [&](int w) {
 #pragma unroll
-            for (int j = 0; j < V; ++j) { v[j] = a.e[j]; v[V + j] = b.e[j]; }
-#pragma unroll
-            for (int j = 0; j < V; ++j) {
-                T& lo = INTER ? v[2 * j] : v[j];
-                T& hi = INTER ? v[2 * j + 1] : v[V + j];
-                const float x = elem_to_f32<T>(lo), y = elem_to_f32<T>(hi);
-                lo = elem_from_f32<T>(x * cs[j] - y * sn[j]);
-                hi = elem_from_f32<T>(x * sn[j] + y * cs[j]);
-            }
-#pragma unroll
-            for (int j = 0; j < V; ++j) { a.e[j] = v[j]; b.e[j] = v[V + j]; }
+        for (int i = 0; i < H; ++i) {
+            dst[i] = nullptr;
+            if (w + i * step >= rows) continue;
+            const int t = (w + i * step) / p.heads, h = w + i * step - t * p.heads;
+            const bool is_q = h < p.hq;
+            const T* src = is_q ? (const T*)p.q + (t0 + t) * p.q_stride + (size_t)h * p.d
+                                : (const T*)p.k + (t0 + t) * p.k_stride + (size_t)(h - p.hq) * p.d;
+            T* to = is_q ? (T*)p.q_out + (t0 + t) * p.q_out_stride + (size_t)h * p.d
+                         : (T*)p.k_out + (t0 + t) * p.k_out_stride + (size_t)(h - p.hq) * p.d;
+            if (!turn && src == to) continue;
+            dst[i] = to;
+            at[i] = t * pairs;
+            a[i] = *reinterpret_cast<const W*>(src + i0);
+            b[i] = *reinterpret_cast<const W*>(src + i1);
         }
-        *reinterpret_cast<W*>(dst + i0) = a;
-        *reinterpret_cast<W*>(dst + i1) = b;
+    };
+    fetch(w0);
+    for (int i = threadIdx.x; i < tokens * pairs; i += kRopeThreads) {
+        const int t = i / pairs;
+        const uint64_t pos = (uint64_t)(int64_t)p.pos[t0 + t];
+        const int32_t part = (int32_t)((pos * p.turns[i - t * pairs]) >> 32);
+        float s, c;
+        sincospif((float)part * (1.0f / 2147483648.0f), &s, &c);
+        sm_cos[i] = c * p.mult;
+        sm_sin[i] = s * p.sign * p.mult;
+    }
+    __syncthreads();
+    for (int w = w0; w < rows; w += H * step) {
+        if (w > w0) fetch(w);
+#pragma unroll
+        for (int i = 0; i < H; ++i) {
+            if (!dst[i]) continue;
+            if (turn) {
+                constexpr int F = V < 4 ? V : 4;
+                float cs[V], sn[V];
+#pragma unroll
+                for (int j = 0; j < V; j += F) {
+                    const Vec<float, F> vc = *reinterpret_cast<const Vec<float, F>*>(sm_cos + at[i] + V * u + j);
+                    const Vec<float, F> vs = *reinterpret_cast<const Vec<float, F>*>(sm_sin + at[i] + V * u + j);
+#pragma unroll
+                    for (int e = 0; e < F; ++e) { cs[j + e] = vc.e[e]; sn[j + e] = vs.e[e]; }
+                }
+                T v[2 * V];
+#pragma unroll
+                for (int j = 0; j < V; ++j) { v[j] = a[i].e[j]; v[V + j] = b[i].e[j]; }
+#pragma unroll
+                for (int j = 0; j < V; ++j) {
+                    T& lo = INTER ? v[2 * j] : v[j];
+                    T& hi = INTER ? v[2 * j + 1] : v[V + j];
+                    const float x = elem_to_f32<T>(lo), y = elem_to_f32<T>(hi);
+                    lo = elem_from_f32<T>(x * cs[j] - y * sn[j]);
+                    hi = elem_from_f32<T>(x * sn[j] + y * cs[j]);
+                }
+#pragma unroll
+                for (int j = 0; j < V; ++j) { a[i].e[j] = v[j]; b[i].e[j] = v[V + j]; }
+            }
+            *reinterpret_cast<W*>(dst[i] + i0) = a[i];
+            *reinterpret_cast<W*>(dst[i] + i1) = b[i];
+        }
     }
 }
 
@@ -95,13 +135,18 @@ static cudaError_t rope_launch(RopeParams p, size_t tokens, bool inter, uintptr_
         v = p.rot % 4 == 0 && (p.d - p.rot) % 4 == 0 && v >= 2 ? 2 : 1;
     p.units = p.d / (2 * v);
     p.rot_units = p.rot / (2 * v);
-    constexpr int threads = 256;   // units <= 256: d <= 512
-    // few tokens: slices of the heads, so that every SM has a CTA
-    const int per = threads / p.units;
+    // four tokens a CTA, as far as their angles fit and every SM still gets eight CTAs; with fewer
+    // tokens than that, slices of the heads
+    const size_t want = 8 * (size_t)device_sm_count();
+    p.tokens = tokens;
+    p.group = 1;
+    while (p.group < 4 && 2 * p.group * (p.rot / 2) <= kRopePairs && tokens / (2 * p.group) >= want) p.group *= 2;
+    const int per = kRopeThreads / p.units;
     const int most = (p.heads + per - 1) / per;
-    size_t slices = tokens >= 4 * (size_t)device_sm_count() ? 1 : (4 * (size_t)device_sm_count() + tokens - 1) / tokens;
+    size_t slices = tokens >= want ? 1 : (want + tokens - 1) / tokens;
     if (slices > (size_t)most) slices = most;
-    const dim3 grid((unsigned)tokens, (unsigned)slices);
+    const dim3 grid((unsigned)((tokens + p.group - 1) / p.group), (unsigned)slices);
+    constexpr int threads = kRopeThreads;
     constexpr int F = 16 / (int)sizeof(T);
     if (inter)
         return v == F ? launch_pdl(rope_kernel<T, F, true>, grid, dim3(threads), 0, st, p)

@@ -22,25 +22,37 @@ __global__ void __launch_bounds__(256) tree_combine_kernel(const TreeParams p) {
     const int n = (total + p.split_tokens - 1) / p.split_tokens;
     if (n <= 1) return;
     const size_t row = (size_t)row0 * p.hq + (size_t)r;
-    const float* ml = p.part_ml + row * p.max_splits * 2;
+    const float2* ml = reinterpret_cast<const float2*>(p.part_ml) + row * p.max_splits;
     float M = kTreeLowest;
-    for (int s = lane; s < n; s += 32) M = fmaxf(M, ml[2 * s]);
+    for (int s = lane; s < n; s += 32) M = fmaxf(M, ml[s].x);
     M = warp_max(M);
+    const float* part = p.part_o + row * p.max_splits * p.d;
+    // 32 pieces at a time, a lane holding the weight of one; four pieces' loads in flight
     float L = 0.f;
-    for (int s = 0; s < n; ++s) L += ml[2 * s + 1] * tree_ex2(ml[2 * s] - M);
-    const float inv = L == 0.f ? 0.f : 1.0f / L;
-    for (int e = lane * 4; e < p.d; e += 128) {
-        float4 acc = {0.f, 0.f, 0.f, 0.f};
-        for (int s = 0; s < n; ++s) {
-            const float f = tree_ex2(ml[2 * s] - M);
-            const float4 v = *reinterpret_cast<const float4*>(p.part_o + (row * p.max_splits + s) * p.d + e);
-            acc.x += v.x * f; acc.y += v.y * f; acc.z += v.z * f; acc.w += v.w * f;
+    float4 acc[2] = {};
+    for (int s0 = 0; s0 < n; s0 += 32) {
+        const float2 mine = s0 + lane < n ? ml[s0 + lane] : make_float2(kTreeLowest, 0.f);
+        const float w = tree_ex2(mine.x - M);
+        L += warp_sum(mine.y * w);
+        const int k = min(32, n - s0);
+#pragma unroll 4
+        for (int s = 0; s < k; ++s) {
+            const float f = __shfl_sync(0xffffffffu, w, s);
+#pragma unroll
+            for (int x = 0; x < 2; ++x) {
+                const int e = lane * 4 + 128 * x;
+                if (e < p.d) {
+                    const float4 v = *reinterpret_cast<const float4*>(part + (size_t)(s0 + s) * p.d + e);
+                    acc[x].x += v.x * f; acc[x].y += v.y * f; acc[x].z += v.z * f; acc[x].w += v.w * f;
+                }
+            }
         }
-        const size_t at = row * p.d + e;
-        tree_store(p.out, p.q_type, at, L == 0.f ? 0.f : acc.x * inv);
-        tree_store(p.out, p.q_type, at + 1, L == 0.f ? 0.f : acc.y * inv);
-        tree_store(p.out, p.q_type, at + 2, L == 0.f ? 0.f : acc.z * inv);
-        tree_store(p.out, p.q_type, at + 3, L == 0.f ? 0.f : acc.w * inv);
+    }
+    const float inv = L == 0.f ? 0.f : 1.0f / L;
+#pragma unroll
+    for (int x = 0; x < 2; ++x) {
+        const int e = lane * 4 + 128 * x;
+        if (e < p.d) tree_store4(p.out, p.q_type, row * p.d + e, acc[x], inv, L == 0.f);
     }
 }
 

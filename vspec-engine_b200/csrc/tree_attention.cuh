@@ -49,15 +49,39 @@ __device__ __forceinline__ int tree_rows(const TreeParams& p, int b, int& row0) 
     return row0 < 0 || row0 >= end ? 0 : min(end - row0, p.max_q);
 }
 
-__device__ __forceinline__ float tree_load(const void* p, int type, size_t i) {
-    if (type == VSPEC_B200_T_F32) return reinterpret_cast<const float*>(p)[i];
-    if (type == VSPEC_B200_T_F16) return __half2float(reinterpret_cast<const __half*>(p)[i]);
-    return __bfloat162float(reinterpret_cast<const __nv_bfloat16*>(p)[i]);
+// N (2, 4 or 8) consecutive values of q from element i on (i a multiple of N).
+template <int N>
+__device__ __forceinline__ void tree_load(const void* p, int type, size_t i, float (&v)[N]) {
+    if (type == VSPEC_B200_T_F32) {
+        constexpr int M = N < 4 ? N : 4;
+#pragma unroll
+        for (int x = 0; x < N; x += M) {
+            const Vec<float, M> w = *reinterpret_cast<const Vec<float, M>*>(reinterpret_cast<const float*>(p) + i + x);
+#pragma unroll
+            for (int e = 0; e < M; ++e) v[x + e] = w.e[e];
+        }
+    } else if (type == VSPEC_B200_T_F16) {
+        const Vec<__half, N> w = *reinterpret_cast<const Vec<__half, N>*>(reinterpret_cast<const __half*>(p) + i);
+#pragma unroll
+        for (int e = 0; e < N; ++e) v[e] = __half2float(w.e[e]);
+    } else {
+        const Vec<__nv_bfloat16, N> w = *reinterpret_cast<const Vec<__nv_bfloat16, N>*>(reinterpret_cast<const __nv_bfloat16*>(p) + i);
+#pragma unroll
+        for (int e = 0; e < N; ++e) v[e] = __bfloat162float(w.e[e]);
+    }
 }
-__device__ __forceinline__ void tree_store(void* p, int type, size_t i, float v) {
-    if (type == VSPEC_B200_T_F32) reinterpret_cast<float*>(p)[i] = v;
-    else if (type == VSPEC_B200_T_F16) reinterpret_cast<__half*>(p)[i] = __float2half_rn(v);
-    else reinterpret_cast<__nv_bfloat16*>(p)[i] = __float2bfloat16_rn(v);
+// Four values v * inv in a row (0 for a row that saw nothing), rounded once.
+__device__ __forceinline__ void tree_store4(void* p, int type, size_t i, float4 v, float inv, bool empty) {
+    v = empty ? make_float4(0.f, 0.f, 0.f, 0.f) : make_float4(v.x * inv, v.y * inv, v.z * inv, v.w * inv);
+    if (type == VSPEC_B200_T_F32) {
+        *reinterpret_cast<float4*>(reinterpret_cast<float*>(p) + i) = v;
+    } else if (type == VSPEC_B200_T_F16) {
+        Vec<__half, 4> w = {{__float2half_rn(v.x), __float2half_rn(v.y), __float2half_rn(v.z), __float2half_rn(v.w)}};
+        *reinterpret_cast<Vec<__half, 4>*>(reinterpret_cast<__half*>(p) + i) = w;
+    } else {
+        Vec<__nv_bfloat16, 4> w = {{__float2bfloat16_rn(v.x), __float2bfloat16_rn(v.y), __float2bfloat16_rn(v.z), __float2bfloat16_rn(v.w)}};
+        *reinterpret_cast<Vec<__nv_bfloat16, 4>*>(reinterpret_cast<__nv_bfloat16*>(p) + i) = w;
+    }
 }
 
 // Whether row i of the tree (first mask row of the sequence: row0) sees the cached token at position t.

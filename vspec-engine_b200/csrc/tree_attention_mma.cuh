@@ -131,20 +131,28 @@ __global__ void __launch_bounds__(kTreeThreads) tree_mma_kernel(const TreeParams
 
     // ---- q rows: power-of-two scale, fp16 parts, swizzled (chunk x of row r at x ^ (r & 7)) ----
     {
-        constexpr int E = D / 32;
-        for (int r = warp; r < MT; r += 4) {
-            const int pr = rt * MT + r;
-            float v[E];
-            float top = 0.f;
-            const bool in = pr < rows;
-            const size_t base = in ? (size_t)(row0 + pr / p.group) * p.q_stride +
-                                         (size_t)(kvh * p.group + pr % p.group) * p.d : 0;
+        constexpr int E = D / 32, B = 4;             // values a lane and row; rows with loads in flight
+        float q[B][E];
+#pragma unroll 1
+        for (int r0 = warp; r0 < MT; r0 += 4 * B) {
 #pragma unroll
-            for (int e = 0; e < E; ++e) {
-                const int i = lane * E + e;
-                v[e] = in && i < p.d ? tree_load(p.q, p.q_type, base + i) : 0.f;
-                top = fmaxf(top, fabsf(v[e]));
+        for (int x = 0; x < B; ++x) {
+            const int pr = rt * MT + r0 + 4 * x;
+            if (pr < rows && lane * E < p.d) {
+                tree_load<E>(p.q, p.q_type, (size_t)(row0 + pr / p.group) * p.q_stride +
+                             (size_t)(kvh * p.group + pr % p.group) * p.d + lane * E, q[x]);
+            } else {
+#pragma unroll
+                for (int e = 0; e < E; ++e) q[x][e] = 0.f;
             }
+        }
+#pragma unroll
+        for (int x = 0; x < B; ++x) {
+            const int r = r0 + 4 * x;
+            float (&v)[E] = q[x];
+            float top = 0.f;
+#pragma unroll
+            for (int e = 0; e < E; ++e) top = fmaxf(top, fabsf(v[e]));
             float mul = 1.0f;
             if (p.q_type != VSPEC_B200_T_F16) {
                 top = warp_max(top);
@@ -172,6 +180,7 @@ __global__ void __launch_bounds__(kTreeThreads) tree_mma_kernel(const TreeParams
 #pragma unroll
                 for (int e = 0; e < E / 2; ++e) reinterpret_cast<uint32_t*>(dst)[e] = w[e];
             }
+        }
         }
     }
     __syncthreads();
@@ -481,12 +490,7 @@ __global__ void __launch_bounds__(kTreeThreads) tree_mma_kernel(const TreeParams
         }
         const size_t orow = (size_t)(row0 + pr / p.group) * p.hq + (size_t)kvh * p.group + pr % p.group;
         if (nsplit == 1) {
-            const float inv = L == 0.f ? 0.f : 1.0f / L;
-            const size_t at = orow * p.d + e;
-            tree_store(p.out, p.q_type, at, L == 0.f ? 0.f : acc.x * inv);
-            tree_store(p.out, p.q_type, at + 1, L == 0.f ? 0.f : acc.y * inv);
-            tree_store(p.out, p.q_type, at + 2, L == 0.f ? 0.f : acc.z * inv);
-            tree_store(p.out, p.q_type, at + 3, L == 0.f ? 0.f : acc.w * inv);
+            tree_store4(p.out, p.q_type, orow * p.d + e, acc, L == 0.f ? 0.f : 1.0f / L, L == 0.f);
         } else {
             const size_t at = orow * p.max_splits + split;
             *reinterpret_cast<float4*>(p.part_o + at * p.d + e) = acc;
