@@ -447,6 +447,9 @@ typedef struct VspecB200TreeAttnArgs {
 size_t vspec_b200_tree_attention_workspace_bytes(size_t batch, size_t total_q, size_t max_q, size_t num_q_heads,
                                                  size_t num_kv_heads, size_t head_dim, size_t max_ctx);
 int vspec_b200_tree_attention(const VspecB200TreeAttnArgs* args, void* stream);
+/* Reads and clears the flag a tree attention launch raises when one of its
+ * bounded waits gave up (1 = seen since the last call; out is incomplete). */
+int vspec_b200_tree_attention_timeout_flag(int* out_flag);
 
 /*
  * Log probabilities from logits, p = softmax(x * inv_temperature) over the

@@ -18,7 +18,7 @@
 
 namespace vb200 {
 
-constexpr int kLpThreads = 512;
+constexpr int kLpThreads = 256;
 constexpr int kLpWarps = kLpThreads / 32;
 constexpr int kLpMaxTop = 32;
 constexpr int kLpCandidates = 2048;
@@ -176,7 +176,7 @@ __device__ __forceinline__ LpStats lp_join_cta(LpShared& sm, LpStats st, float c
 // largest of the threads' maxima, below which no value can be among the best.
 // At most 32 threads (top_k <= 32) then add their U * V values.
 template <typename T, int V, bool ALLOWED, bool TOP>
-__global__ void __launch_bounds__(kLpThreads, 2) logprobs_kernel(const LpParams p) {
+__global__ void __launch_bounds__(kLpThreads, 4) logprobs_kernel(const LpParams p) {
     pdl_wait();
     pdl_trigger();
     constexpr int U = 16 / V;   // vectors a thread and block (16 values: more spill)
@@ -393,13 +393,13 @@ __global__ void __launch_bounds__(kLpThreads, 2) logprobs_kernel(const LpParams 
     }
 }
 
-// CTAs a row: what fills the two resident on every SM, each with at least 4096
+// CTAs a row: what fills the four resident on every SM, each with at least 2048
 // values. A row's fixed cost (two selections) is why rows that fill the SMs
 // are not split for a better balance.
 static int lp_splits(size_t rows, size_t vocab) {
     if (rows >= (size_t)kLpMaxSplitRows) return 1;
-    size_t s = 2 * (size_t)device_sm_count() / rows;
-    const size_t most = vocab / 4096;
+    size_t s = 4 * (size_t)device_sm_count() / rows;
+    const size_t most = vocab / 2048;
     if (s > most) s = most;
     return s < 1 ? 1 : (int)s;
 }

@@ -1,7 +1,7 @@
 // tree_attention.cu -- entry point of the tree attention: argument checks, the
 // plan (rows and context of a CTA) and the kernel that joins context pieces.
 #include "attention_kernels.cuh"
-#include "tree_attention_mma.cuh"
+#include "tree_attention_tc.cuh"
 
 #include <limits.h>
 #include <string.h>
@@ -56,16 +56,48 @@ __global__ void __launch_bounds__(256) tree_combine_kernel(const TreeParams p) {
     }
 }
 
+__device__ int g_tree_timeout = 0;
+
+static int* tree_timeout_ptr() {
+    static int* ptr[64] = {};
+    int dev = 0;
+    if (cudaGetDevice(&dev) != cudaSuccess || dev < 0 || dev >= 64) return nullptr;
+    if (!ptr[dev]) {
+        void* p = nullptr;
+        if (cudaGetSymbolAddress(&p, g_tree_timeout) != cudaSuccess) return nullptr;
+        ptr[dev] = reinterpret_cast<int*>(p);
+    }
+    return ptr[dev];
+}
+
 struct TreePlan {
-    int wr, row_tiles, split_tokens, max_splits;
+    bool tc;
+    int ctas;                                          // tcgen05 kernel
+    int wr, row_tiles, split_tokens, max_splits;       // warp-MMA kernel
 };
 
-// Rows a CTA: 16, 32 or 64, the fewest that hold a pair's rows.  Context
+// Rows a pair has at most: its drafted tokens times the group's heads.  From 33
+// rows on the tcgen05 kernel; below, its 128-row tiles are mostly padding and the
+// warp-MMA kernel reads the cache as fast.  Heads above 128 do not fit its
+// registers (a row's output a thread), pages of other than 8 k tokens its TMA boxes.
+static bool tree_uses_tc(long long rows, size_t d, size_t page_tokens) {
+    return rows > 32 && d <= 128 && page_tokens % 8 == 0;
+}
+
+// Warp-MMA: rows a CTA 16, 32 or 64, the fewest that hold a pair's rows; context
 // pieces: about four CTAs for each that is resident at once (sequences differ
 // in length), at least 128 tokens each.
-static TreePlan tree_plan(size_t batch, size_t max_q, size_t hq, size_t hkv, size_t max_ctx) {
-    TreePlan t;
+static TreePlan tree_plan(size_t batch, size_t max_q, size_t hq, size_t hkv, size_t d, size_t page_tokens, size_t max_ctx) {
+    TreePlan t = {};
     const long long rows = (long long)max_q * (long long)(hq / hkv);
+    t.tc = tree_uses_tc(rows, d, page_tokens);
+    if (t.tc) {
+        const long long steps = (long long)batch * hkv * ((rows + 127) / 128) * (((long long)max_ctx + kTcStep - 1) / kTcStep);
+        const long long most = device_sm_count();
+        t.ctas = (int)((steps + 1) / 2 < most ? (steps + 1) / 2 : most);
+        t.max_splits = 1;
+        return t;
+    }
     t.wr = rows <= 16 ? 1 : (rows <= 32 ? 2 : 4);
     t.row_tiles = (int)((rows + 16 * t.wr - 1) / (16 * t.wr));
     const long long pairs = (long long)batch * hkv * t.row_tiles;
@@ -79,8 +111,10 @@ static TreePlan tree_plan(size_t batch, size_t max_q, size_t hq, size_t hkv, siz
     return t;
 }
 
-static size_t tree_workspace(const TreePlan& t, size_t total_q, size_t hq, size_t d) {
-    return t.max_splits > 1 ? total_q * hq * (size_t)t.max_splits * (d + 2) * sizeof(float) : 0;
+// Part slots of the plan: (O, m, l) each.
+static size_t tree_parts(const TreePlan& t, size_t total_q, size_t max_q, size_t hq, size_t hkv) {
+    if (t.tc) return (size_t)2 * t.ctas * (max_q * (hq / hkv) > 128 ? 256 : 128);
+    return t.max_splits > 1 ? total_q * hq * (size_t)t.max_splits : 0;
 }
 
 // Library-managed scratch, one grow-only buffer per device and host thread.
@@ -108,12 +142,24 @@ static void* tree_scratch(size_t bytes) {
 
 using namespace vb200;
 
+extern "C" int vspec_b200_tree_attention_timeout_flag(int* out_flag) {
+    if (!out_flag) { set_error("NULL out_flag"); return VSPEC_B200_ERR_ARG; }
+    int v = 0, zero = 0;
+    VB_CHECK_CUDA(cudaMemcpyFromSymbol(&v, g_tree_timeout, sizeof(int)));
+    VB_CHECK_CUDA(cudaMemcpyToSymbol(g_tree_timeout, &zero, sizeof(int)));
+    *out_flag = v;
+    return VSPEC_B200_OK;
+}
+
 extern "C" size_t vspec_b200_tree_attention_workspace_bytes(size_t batch, size_t total_q, size_t max_q, size_t hq,
                                                             size_t hkv, size_t d, size_t max_ctx) {
     if (batch == 0 || max_q == 0 || hq == 0 || hkv == 0 || hq % hkv != 0 || d == 0 || max_ctx == 0 ||
         max_ctx > (size_t)INT_MAX || batch > 65535 || max_q > (size_t)INT_MAX / hq)
         return 0;
-    return tree_workspace(tree_plan(batch, max_q, hq, hkv, max_ctx), total_q, hq, d);
+    // the larger of the two kernels' (the page size decides between them)
+    const size_t a = tree_parts(tree_plan(batch, max_q, hq, hkv, d, 8, max_ctx), total_q, max_q, hq, hkv);
+    const size_t b = tree_parts(tree_plan(batch, max_q, hq, hkv, d, 1, max_ctx), total_q, max_q, hq, hkv);
+    return (a > b ? a : b) * (d + 2) * sizeof(float);
 }
 
 extern "C" int vspec_b200_tree_attention(const VspecB200TreeAttnArgs* a, void* stream) {
@@ -154,7 +200,7 @@ extern "C" int vspec_b200_tree_attention(const VspecB200TreeAttnArgs* a, void* s
     if (al % 16 != 0) { set_error("q, out, pages and scales must be 16-byte aligned"); return VSPEC_B200_ERR_ARG; }
     if (a->total_q == 0) return VSPEC_B200_OK;
 
-    const TreePlan plan = tree_plan(a->batch, a->max_q, a->num_q_heads, a->num_kv_heads, max_ctx);
+    const TreePlan plan = tree_plan(a->batch, a->max_q, a->num_q_heads, a->num_kv_heads, a->head_dim, a->page_tokens, max_ctx);
     TreeParams p;
     memset(&p, 0, sizeof(p));
     p.q = a->d_q;
@@ -176,7 +222,8 @@ extern "C" int vspec_b200_tree_attention(const VspecB200TreeAttnArgs* a, void* s
     if ((size_t)p.hkv * p.row_tiles > 65535) { set_error("a size is too large"); return VSPEC_B200_ERR_ARG; }
     p.fault = attn_page_fault_device_ptr();
     if (!p.fault) return cuda_status(cudaGetLastError(), "page fault flag");
-    const size_t need = tree_workspace(plan, a->total_q, a->num_q_heads, a->head_dim);
+    const size_t parts = tree_parts(plan, a->total_q, a->max_q, a->num_q_heads, a->num_kv_heads);
+    const size_t need = parts * (a->head_dim + 2) * sizeof(float);
     if (need) {
         void* ws = a->d_workspace;
         if (ws) {
@@ -187,9 +234,25 @@ extern "C" int vspec_b200_tree_attention(const VspecB200TreeAttnArgs* a, void* s
             if (!ws) { set_error("cannot allocate %zu bytes of scratch", need); return VSPEC_B200_ERR_NOMEM; }
         }
         p.part_o = (float*)ws;
-        p.part_ml = p.part_o + a->total_q * a->num_q_heads * (size_t)p.max_splits * a->head_dim;
+        p.part_ml = p.part_o + parts * a->head_dim;
     }
     cudaStream_t st = (cudaStream_t)stream;
+    if (plan.tc) {
+        TcParams pp;
+        memset(&pp, 0, sizeof(pp));
+        pp.t = p;
+        pp.timeout = tree_timeout_ptr();
+        if (!pp.timeout) return cuda_status(cudaGetLastError(), "timeout flag");
+        pp.box_rows = 8;   // the largest power of two that divides the page, up to a whole step
+        while (pp.box_rows < kTcStep && p.page_tokens % (2 * pp.box_rows) == 0) pp.box_rows *= 2;
+        int rc = tree_tc_map(&pp.k_map, p.k_pages, p, f16, pp.box_rows);
+        if (rc == VSPEC_B200_OK) rc = tree_tc_map(&pp.v_map, p.v_pages, p, f16, pp.box_rows);
+        if (rc != VSPEC_B200_OK) return rc;
+        const cudaError_t e = f16 ? tree_tc_launch<kTreeF16>(pp, plan.ctas, st)
+                            : a->kv_dtype == VSPEC_B200_KV_FP8 ? tree_tc_launch<kTreeFp8>(pp, plan.ctas, st)
+                                                               : tree_tc_launch<kTreeInt8>(pp, plan.ctas, st);
+        return e == cudaSuccess ? VSPEC_B200_OK : cuda_status(e, "tree attention launch");
+    }
     cudaError_t e = f16 ? tree_mma_launch<kTreeF16>(p, plan.wr, st)
                   : a->kv_dtype == VSPEC_B200_KV_FP8 ? tree_mma_launch<kTreeFp8>(p, plan.wr, st)
                                                      : tree_mma_launch<kTreeInt8>(p, plan.wr, st);

@@ -1,0 +1,1051 @@
+// tree_attention_tc.cuh -- tree attention on the 5th-generation tensor cores:
+// many query rows a (sequence, KV head) pair (wide trees, large groups).
+//
+// With R rows a pair, every cached token costs 4 R d operations for 4 d bytes of
+// fp16: from a few dozen rows on, warp-level MMA (576 TFLOP/s here) and not DRAM
+// is the bound.  Here one thread issues tcgen05.mma for tiles of 128 rows x 128
+// tokens, with S = Q K^T and O = P V in tensor memory:
+//   warps 0-3, 4-7   softmax, one thread a row (TMEM lane): maximum and
+//                    exponentials of S, P back over S as fp16, the step's O
+//                    added to fp32 registers (a step's product starts from 0:
+//                    the tensor cores truncate, see tree_attention_mma.cuh)
+//   warp 8           one lane issues the products
+//   warps 9-11       K and V pages into a ring of swizzled 128-token tiles by
+//   (9-15 for 8-bit) TMA boxes (page_tokens a multiple of 8); 8-bit codes land
+//                    in a raw ring and are widened to fp16 into the tiles
+// Two tiles are in flight so that the tensor cores work on one while the other
+// is in its softmax: two row tiles sharing each K and V tile when a pair has
+// more than 128 rows (TILES = 2), else alternate steps of one row tile, joined
+// at the end (TILES = 1).
+//
+// The grid is persistent: all pairs' steps, laid out in a row, are cut into
+// equal runs, one a CTA, so that sequences of any lengths balance to one step.
+// A run that cuts a pair writes that part's (O, m, l); a second kernel joins
+// the parts of such pairs in order.  fp32 q and 8-bit pages are split and scaled
+// as in the warp-MMA kernels.
+#pragma once
+
+#include "tma_map.cuh"
+#include "tree_attention_mma.cuh"
+
+namespace vb200 {
+
+constexpr int kTcMmaWarp = 8, kTcFirstProducer = 9;
+constexpr int kTcStep = 128;
+constexpr long long kTcWaitCycles = 4000000000ll;
+constexpr uint32_t kTcHalf = 128u * 128u;          // 128 rows x 64 fp16
+constexpr int kTcRawSlots = 3;
+constexpr uint32_t kTcSmemMax = 232448u;
+
+struct TcParams {
+    TreeParams t;
+    CUtensorMap k_map, v_map;   // [pool rows][KV heads][d], boxes of box_rows x 1 x 64 values (8-bit: x d)
+    int box_rows;               // divides page_tokens and kTcStep
+    int* timeout;
+};
+
+template <int D, int TILES, int QS, int KV>
+struct TcShape {
+    static constexpr int kProducers = KV == kTreeF16 ? 3 : 7;
+    static constexpr int kThreads = (kTcFirstProducer + kProducers) * 32;
+    // registers a thread of the softmax warps (256 threads) and of the others: together what the CTA is launched
+    // with, 384 x 168 or 512 x 128
+    static constexpr int kSoftmaxRegs = KV == kTreeF16 ? 216 : 192, kOtherRegs = KV == kTreeF16 ? 72 : 64;
+    static_assert(256 * kSoftmaxRegs + (kThreads - 256) * kOtherRegs <= kThreads * (65536 / kThreads / 8 * 8), "register split");
+    static constexpr uint32_t kSlot = kTcStep * D * 2;
+    static constexpr uint32_t kQ = TILES * QS * kSlot;
+    static constexpr uint32_t kRaw = KV == kTreeF16 ? 0 : kTcRawSlots * kTcStep * D;
+    static constexpr uint32_t kMisc = KV == kTreeF16 ? 3072 : 7168;
+    static constexpr int kFit = (int)((kTcSmemMax - kMisc - kQ - kRaw) / kSlot);
+    static constexpr int kMost = KV == kTreeF16 ? 6 : 4;   // 4: the scale ring below
+    static constexpr int kSlots = kFit < kMost ? kFit : kMost;
+    static constexpr uint32_t kRingAt = kQ, kRawAt = kQ + kSlots * kSlot, kMiscAt = kRawAt + kRaw;
+    static constexpr uint32_t kTotal = kMiscAt + kMisc;
+    static_assert(kSlots >= 3, "ring");
+};
+
+// misc area
+struct alignas(16) TcMisc {
+    float mul[256];             // score multiplier of each row
+    uint64_t full[6], empty[6], raw_full[kTcRawSlots], raw_empty[kTcRawSlots], s_full[2], p_full[2], q_full, pair, staged[2], drain;
+    uint32_t tmem;
+    int abort;
+    int start_b;
+    long long start_off, total;
+    int odd[8];                 // step + 1 where V held infinities or NaN
+    float ml[2][128];           // of the second softmax group (TILES = 1)
+};
+struct alignas(16) TcScales {   // 8-bit pages: scales of four steps, read four at a time
+    float k[4][kTcStep], v[4][kTcStep];
+    float one[kTcStep];
+    int v_exp[4];
+};
+__device__ __forceinline__ void tc_tma_3d(uint32_t dst, const CUtensorMap* map, int x, int y, int z, uint64_t* bar) {
+    asm volatile(
+        "cp.async.bulk.tensor.3d.shared::cluster.global.mbarrier::complete_tx::bytes [%0], [%1, {%2, %3, %4}], [%5];\n"
+        ::"r"(dst), "l"(reinterpret_cast<uint64_t>(map)), "r"(x), "r"(y), "r"(z), "r"(smem_u32(bar)) : "memory");
+}
+
+__device__ __forceinline__ void tc_st_x16(uint32_t taddr, const uint32_t (&v)[16]) {
+    asm volatile(
+        "tcgen05.st.sync.aligned.32x32b.x16.b32 [%0], "
+        "{%1,%2,%3,%4,%5,%6,%7,%8,%9,%10,%11,%12,%13,%14,%15,%16};\n"
+        ::"r"(taddr), "r"(v[0]), "r"(v[1]), "r"(v[2]), "r"(v[3]), "r"(v[4]), "r"(v[5]), "r"(v[6]), "r"(v[7]),
+          "r"(v[8]), "r"(v[9]), "r"(v[10]), "r"(v[11]), "r"(v[12]), "r"(v[13]), "r"(v[14]), "r"(v[15])
+        : "memory");
+}
+__device__ __forceinline__ void tc_st_x8(uint32_t taddr, const uint32_t (&v)[8]) {
+    asm volatile("tcgen05.st.sync.aligned.32x32b.x8.b32 [%0], {%1,%2,%3,%4,%5,%6,%7,%8};\n"
+                 ::"r"(taddr), "r"(v[0]), "r"(v[1]), "r"(v[2]), "r"(v[3]), "r"(v[4]), "r"(v[5]), "r"(v[6]), "r"(v[7])
+                 : "memory");
+}
+// Shared-memory operands, 128-byte swizzle, as the two words of their
+// descriptors: low = address >> 4 (14 bits) | leading offset >> 4 << 16, high =
+// stride offset 1024 >> 4 | version 1 << 14 | swizzle 2 << 29.
+//   K-major (Q, K): rows of 64 values, 8-row groups 1024 bytes apart.
+//   N-major (V: tokens are K, dims N): 64 dims a 128-byte row, 8 tokens 1024
+//   bytes, the next 64 dims kTcHalf bytes on (the leading offset).
+constexpr uint32_t kTcDescHigh = (1024u >> 4) | (1u << 14) | (2u << 29);
+constexpr uint32_t kTcLeadK = 1u << 16, kTcLeadV = (kTcHalf >> 4) << 16;
+// D[tmem] (+)= A[smem] * B[smem], issued by one thread.
+__device__ __forceinline__ void tc_mma_ss(uint32_t d_taddr, uint32_t a_low, uint32_t b_low, uint32_t idesc, uint32_t acc) {
+    asm volatile(
+        "{\n.reg .pred p;\n.reg .b64 da, db;\nsetp.ne.u32 p, %4, 0;\nmov.b64 da, {%1, %5};\nmov.b64 db, {%2, %5};\n"
+        "tcgen05.mma.cta_group::1.kind::f16 [%0], da, db, %3, p;\n}\n"
+        ::"r"(d_taddr), "r"(a_low), "r"(b_low), "r"(idesc), "r"(acc), "r"(kTcDescHigh) : "memory");
+}
+// The same with A in tensor memory.
+__device__ __forceinline__ void tc_mma_ts(uint32_t d_taddr, uint32_t a_taddr, uint32_t b_low, uint32_t idesc, uint32_t acc) {
+    asm volatile(
+        "{\n.reg .pred p;\n.reg .b64 db;\nsetp.ne.u32 p, %4, 0;\nmov.b64 db, {%2, %5};\n"
+        "tcgen05.mma.cta_group::1.kind::f16 [%0], [%1], db, %3, p;\n}\n"
+        ::"r"(d_taddr), "r"(a_taddr), "r"(b_low), "r"(idesc), "r"(acc), "r"(kTcDescHigh) : "memory");
+}
+template <int N>
+__device__ __forceinline__ void tc_regs_inc() { asm volatile("setmaxnreg.inc.sync.aligned.u32 %0;\n" ::"n"(N)); }
+template <int N>
+__device__ __forceinline__ void tc_regs_dec() { asm volatile("setmaxnreg.dec.sync.aligned.u32 %0;\n" ::"n"(N)); }
+
+// Waits for this warp's TMEM loads; v is what one of them returned, so that no
+// use of it can be moved in front of the wait.
+__device__ __forceinline__ void tc_landed(float (&v)[16]) {
+    asm volatile("tcgen05.wait::ld.sync.aligned;\n"
+                 : "+f"(v[0]), "+f"(v[1]), "+f"(v[2]), "+f"(v[3]), "+f"(v[4]), "+f"(v[5]), "+f"(v[6]), "+f"(v[7]),
+                   "+f"(v[8]), "+f"(v[9]), "+f"(v[10]), "+f"(v[11]), "+f"(v[12]), "+f"(v[13]), "+f"(v[14]), "+f"(v[15])
+                 :: "memory");
+}
+// f(c, v) for N chunks of 16 TMEM columns of this thread's lane, the next chunk's load in flight.
+template <int N, typename F>
+__device__ __forceinline__ void tc_sweep(uint32_t taddr, F f) {
+    static_assert(N % 2 == 0, "pairs of chunks");
+    float a[16], b[16];
+    tmem_ld_x16(taddr, a);
+#pragma unroll
+    for (int c = 0; c < N; c += 2) {
+        tc_landed(a);
+        tmem_ld_x16(taddr + 16u * (c + 1), b);
+        f(c, a);
+        tc_landed(b);
+        if (c + 2 < N) tmem_ld_x16(taddr + 16u * (c + 2), a);
+        f(c + 1, b);
+    }
+}
+template <bool ON>
+__device__ __forceinline__ void tc_scale(float (&v)[16], const float* s) {
+#pragma unroll
+    for (int x = 0; ON && x < 16; x += 4) {
+        const float4 k = *reinterpret_cast<const float4*>(s + x);
+        v[x] *= k.x; v[x + 1] *= k.y; v[x + 2] *= k.z; v[x + 3] *= k.w;
+    }
+}
+
+// Wait bounded by time (about two seconds).
+__device__ __forceinline__ bool tc_wait_one(uint64_t* bar, uint32_t parity, volatile int* abort) {
+    if (mbar_try_wait(bar, parity)) return true;
+    const long long start = clock64();
+    while (!mbar_try_wait(bar, parity))
+        if (*abort || clock64() - start > kTcWaitCycles) return false;
+    return true;
+}
+// The same for a whole warp, with one answer for all its lanes.
+__device__ __forceinline__ bool tc_wait(uint64_t* bar, uint32_t parity, volatile int* abort) {
+    return __all_sync(0xffffffffu, tc_wait_one(bar, parity, abort));
+}
+
+// ---- the work: sequence b has pairs (KV head, row tile) of n steps each ----
+template <int RT>
+__device__ __forceinline__ long long tc_work(const TreeParams& p, int b, int& n, int& tiles) {
+    int row0;
+    const int drafted = tree_rows(p, b, row0);
+    const int total = max(p.ctx_len[b], 0) + drafted;
+    n = (total + kTcStep - 1) / kTcStep;
+    tiles = (drafted * p.group + RT - 1) / RT;
+    return drafted ? (long long)n * p.hkv * tiles : 0;
+}
+// CTAs that take part: at least two steps each.
+__device__ __forceinline__ int tc_ctas(long long total, int most) {
+    const long long g = (total + 1) / 2;
+    return (int)(g < 1 ? 1 : (g < most ? g : most));
+}
+
+// A run of steps within one pair.
+struct TcSegment {
+    int b, row0, drafted, ctx, kvh, rt, n, step0, steps;
+};
+template <int RT>
+struct TcWalk {
+    int b;
+    long long off, left;
+    // the next segment of the CTA's run, or false
+    __device__ __forceinline__ bool next(const TreeParams& p, TcSegment& s) {
+        while (left > 0) {
+            int n, tiles;
+            const long long w = tc_work<RT>(p, b, n, tiles);
+            if (off >= w) { off -= w; ++b; continue; }
+            s.b = b;
+            s.drafted = tree_rows(p, b, s.row0);
+            s.ctx = max(p.ctx_len[b], 0);
+            s.n = n;
+            const long long pair = off / n;
+            s.step0 = (int)(off - pair * n);
+            s.kvh = (int)(pair / tiles);
+            s.rt = (int)(pair - (long long)s.kvh * tiles);
+            s.steps = (int)min((long long)(n - s.step0), left);
+            off += s.steps;
+            left -= s.steps;
+            return true;
+        }
+        return false;
+    }
+};
+
+// Eight fp16 values with infinities and NaN replaced by 0.
+__device__ __forceinline__ void tc_clear_odd(uint4& v) {
+    uint32_t* w = reinterpret_cast<uint32_t*>(&v);
+#pragma unroll
+    for (int e = 0; e < 4; ++e) {
+        if ((w[e] & 0x7C00u) == 0x7C00u) w[e] &= 0xFFFF0000u;
+        if ((w[e] & 0x7C000000u) == 0x7C000000u) w[e] &= 0x0000FFFFu;
+    }
+}
+
+// Bits of the drafted tokens j0 .. j0 + 31 (j0 < 0: committed ones) that token i of the tree sees.
+__device__ __forceinline__ uint32_t tc_sees32(const TreeParams& p, int row0, int i, int drafted, int j0) {
+    auto word = [&](int k) -> uint32_t {
+        if (k < 0) return 0xffffffffu;
+        const int left = drafted - 32 * k;
+        if (left <= 0) return 0u;
+        uint32_t v;
+        if (p.mask) v = __ldg(p.mask + (size_t)(row0 + i) * p.mask_words + k);
+        else v = i - 32 * k >= 31 ? 0xffffffffu : (i < 32 * k ? 0u : (2u << (i - 32 * k)) - 1u);
+        return left < 32 ? v & ((1u << left) - 1u) : v;
+    };
+    const int k = j0 >> 5, sh = j0 & 31;
+    return sh ? (word(k) >> sh) | (word(k + 1) << (32 - sh)) : word(k);
+}
+
+template <int D, int TILES, int QS, int KV>
+__global__ void __launch_bounds__(TcShape<D, TILES, QS, KV>::kThreads, 1) tree_tc_kernel(const __grid_constant__ TcParams pp) {
+    const TreeParams& p = pp.t;
+    using S = TcShape<D, TILES, QS, KV>;
+    constexpr int RT = 128 * TILES, NS = S::kSlots, kTcProducers = S::kProducers;
+    extern __shared__ __align__(1024) unsigned char tc_smem[];
+    unsigned char* const smem = tc_smem;
+    TcMisc& sm = *reinterpret_cast<TcMisc*>(smem + S::kMiscAt);
+    TcScales& sc = *reinterpret_cast<TcScales*>(smem + S::kMiscAt + sizeof(TcMisc));
+    static_assert(sizeof(TcMisc) % 16 == 0 && S::kMiscAt % 16 == 0, "vector reads of the scales behind");
+    static_assert(sizeof(TcMisc) + (KV == kTreeF16 ? 0 : sizeof(TcScales)) <= S::kMisc, "misc area");
+    const int tid = threadIdx.x, warp = tid >> 5, lane = tid & 31;
+    volatile int* abort_flag = &sm.abort;
+    pdl_wait();
+    pdl_trigger();
+
+    // ---- this CTA's run ----
+    if (tid == 0) {
+        sm.abort = 0;
+        for (int i = 0; i < 6; ++i) { mbar_init(&sm.full[i], kTcProducers); mbar_init(&sm.empty[i], 1); }
+        for (int i = 0; i < kTcRawSlots; ++i) { mbar_init(&sm.raw_full[i], 1); mbar_init(&sm.raw_empty[i], kTcProducers); }
+        for (int i = 0; i < 2; ++i) { mbar_init(&sm.s_full[i], 1); mbar_init(&sm.p_full[i], 128); }
+        mbar_init(&sm.q_full, 256);
+        mbar_init(&sm.pair, 256);
+        for (int i = 0; i < 2; ++i) mbar_init(&sm.staged[i], 128);
+        mbar_init(&sm.drain, 1);
+        mbar_fence_init();
+        for (int i = 0; i < 8; ++i) sm.odd[i] = 0;
+        tma_prefetch_desc(&pp.k_map);
+        tma_prefetch_desc(&pp.v_map);
+    }
+    if (KV != kTreeF16 && tid < kTcStep) sc.one[tid] = 1.0f;
+    long long lo = 0, hi = 0;
+    if (warp == 0) {
+        long long total = 0;
+        for (int b0 = 0; b0 < p.batch; b0 += 32) {
+            int n, tiles;
+            long long w = b0 + lane < p.batch ? tc_work<RT>(p, b0 + lane, n, tiles) : 0;
+#pragma unroll
+            for (int o = 16; o > 0; o >>= 1) w += __shfl_xor_sync(0xffffffffu, w, o);
+            total += w;
+        }
+        const int g = tc_ctas(total, gridDim.x);
+        lo = (int)blockIdx.x < g ? total * (int)blockIdx.x / g : total;
+        long long before = 0;
+        int found = -1;
+        for (int b0 = 0; b0 < p.batch && found < 0 && lo < total; b0 += 32) {
+            int n, tiles;
+            const long long w = b0 + lane < p.batch ? tc_work<RT>(p, b0 + lane, n, tiles) : 0;
+            long long incl = w;
+#pragma unroll
+            for (int o = 1; o < 32; o <<= 1) {
+                const long long u = __shfl_up_sync(0xffffffffu, incl, o);
+                if (lane >= o) incl += u;
+            }
+            const unsigned hit = __ballot_sync(0xffffffffu, before + incl > lo);
+            if (hit) {
+                const int at = __ffs(hit) - 1;
+                found = b0 + at;
+                const long long start = before + __shfl_sync(0xffffffffu, incl - w, at);
+                if (lane == 0) { sm.start_b = found; sm.start_off = lo - start; }
+            }
+            before += __shfl_sync(0xffffffffu, incl, 31);
+        }
+        if (lane == 0) sm.total = total;
+    }
+    if (warp == kTcMmaWarp) {
+        tmem_alloc(&sm.tmem, 512);
+        tmem_relinquish();
+    }
+    tc_fence_before();
+    __syncthreads();
+    tc_fence_after();
+    const uint32_t tmem = sm.tmem;
+    TcWalk<RT> walk;
+    {
+        const long long total = sm.total;
+        const int g = tc_ctas(total, gridDim.x);
+        lo = (int)blockIdx.x < g ? total * (int)blockIdx.x / g : total;
+        hi = (int)blockIdx.x < g ? total * ((int)blockIdx.x + 1) / g : total;
+        walk.left = hi - lo;
+        walk.b = walk.left > 0 ? sm.start_b : 0;
+        walk.off = walk.left > 0 ? sm.start_off : 0;
+    }
+    // TMEM columns: S (and P over it) of softmax group w at 128 w, its O at 256 + 128 w
+    TcSegment seg;
+    bool ok = true;
+    if (warp >= kTcMmaWarp) {
+    tc_regs_dec<S::kOtherRegs>();
+    if (warp >= kTcFirstProducer) {
+        // ============================ producers ============================
+        const int pw = warp - kTcFirstProducer;
+        const int br = pp.box_rows, boxes = kTcStep / br;      // boxes of a whole tile: 1 to 16
+        int slot = 0, raw = 0;
+        uint32_t phase = 0, raw_phase = 0;   // of the slot's next use
+        uint32_t raw_used = 0;               // raw slots used before, and from bit 8 the phases of their release
+        bool wrapped = false;                // the ring has been filled once
+        int k_steps = 0;                     // steps of the CTA's run before this segment
+        auto advance = [&]() {
+            if (++slot == NS) { slot = 0; phase ^= 1u; wrapped = true; }
+        };
+        auto wait_slot = [&]() -> bool { return !wrapped || tc_wait(&sm.empty[slot], phase ^ 1u, abort_flag); };
+        // load li of a segment: K or V of its step j, in the order in which the products need them
+        auto decode = [&](int li, bool& is_v, int& j) {
+            if (TILES == 2) { is_v = li & 1; j = li >> 1; }
+            else if (li == 0) { is_v = false; j = 0; }
+            else { is_v = (li & 1) == 0; j = is_v ? (li - 2) >> 1 : (li + 1) >> 1; }
+        };
+        while (ok && walk.next(p, seg)) {
+            const int32_t* table = p.table + (size_t)seg.b * p.max_pages;
+            const int total = seg.ctx + seg.drafted, t_first = seg.step0 * kTcStep;
+            const int loads = TILES == 2 ? 2 * seg.steps : 2 * seg.steps + 1;
+            // pool row of box `lane` of step j, a step ahead of its use
+            auto find = [&](int j) -> int {
+                const int t = t_first + j * kTcStep + lane * br;
+                return j < seg.steps && lane < boxes && t < total ? tree_pool_row(p, table, t) : 0;
+            };
+            int row_even = find(0), row_odd = find(1);
+            // the boxes of K or V of step j
+            auto issue = [&](bool is_v, int j, uint32_t dst, uint64_t* bar) {
+                const int left = total - (t_first + j * kTcStep);
+                const int nb = left >= kTcStep ? boxes : (left + br - 1) / br;
+                constexpr uint32_t kRowBytes = KV == kTreeF16 ? D * 2 : D;
+                if (lane == 0) mbar_arrive_expect_tx(bar, (uint32_t)(nb * br) * kRowBytes);
+                __syncwarp();
+                const int row = (j & 1) ? row_odd : row_even;
+                const CUtensorMap* map = is_v ? &pp.v_map : &pp.k_map;
+                if (lane < nb) {
+                    if (KV == kTreeF16) {
+#pragma unroll
+                        for (int h = 0; h < D / 64; ++h)
+                            tc_tma_3d(dst + h * kTcHalf + (uint32_t)(lane * br) * 128u, map, 64 * h, seg.kvh, row, bar);
+                    } else {
+                        tc_tma_3d(dst + (uint32_t)(lane * br) * D, map, 0, seg.kvh, row, bar);
+                    }
+                }
+                // K and V of a step share its rows: after V they are those of the step after next
+                if (is_v) {
+                    const int next = find(j + 2);
+                    if (j & 1) row_odd = next; else row_even = next;
+                }
+            };
+            const uint32_t ring = smem_u32(smem) + S::kRingAt;
+            if constexpr (KV == kTreeF16) {
+                for (int li = 0; li < loads && ok; ++li) {
+                    bool is_v;
+                    int j;
+                    decode(li, is_v, j);
+                    if (j >= seg.steps) continue;
+                    if (!wait_slot()) { ok = false; break; }
+                    const bool drafted = t_first + (j + 1) * kTcStep > seg.ctx;
+                    if (!(is_v && drafted)) {
+                        if (pw == 0) issue(is_v, j, ring + (uint32_t)slot * S::kSlot, &sm.full[slot]);
+                        else if (lane == 0) mbar_arrive(&sm.full[slot]);
+                    } else {
+                        // V of a step with drafted tokens: what is past the last token becomes 0, and so do infinities and
+                        // NaN, which are noted
+                        if (pw == 0) issue(true, j, ring + (uint32_t)slot * S::kSlot, &sm.raw_full[0]);
+                        if (!tc_wait(&sm.raw_full[0], raw_phase, abort_flag)) { ok = false; break; }
+                        raw_phase ^= 1u;
+                        unsigned char* st = smem + S::kRingAt + (uint32_t)slot * S::kSlot;
+                        const int there = min(total - (t_first + j * kTcStep), kTcStep);
+                        bool odd = false;
+#pragma unroll 4
+                        for (int i = pw * 32 + lane; i < kTcStep * (D / 8); i += kTcProducers * 32) {
+                            uint4* at = reinterpret_cast<uint4*>(st) + i;
+                            const int r = (i >> 3) & (kTcStep - 1);     // 8 chunks a row of each half
+                            if (r >= there) {
+                                *at = make_uint4(0, 0, 0, 0);
+                            } else if (tree_odd_chunk(*at)) {
+                                odd = true;
+                                uint4 v = *at;
+                                tc_clear_odd(v);
+                                *at = v;
+                            }
+                        }
+                        if (odd) sm.odd[(k_steps + j) & 7] = k_steps + j + 1;
+                        asm volatile("fence.proxy.async.shared::cta;\n" ::: "memory");
+                        __syncwarp();
+                        if (lane == 0) mbar_arrive(&sm.full[slot]);
+                    }
+                    advance();
+                }
+            } else {
+                // codes of load li land in raw slot `raw`, three loads ahead of the conversion
+                auto issue_raw = [&](int li, int to) {
+                    bool is_v;
+                    int j;
+                    decode(li, is_v, j);
+                    if (pw == 0 && li < loads && j < seg.steps) {
+                        // every warp has read what the slot held
+                        if ((raw_used >> to) & 1u) {
+                            if (!tc_wait(&sm.raw_empty[to], (raw_used >> (8 + to)) & 1u, abort_flag)) ok = false;
+                            raw_used ^= 256u << to;
+                        }
+                        raw_used |= 1u << to;
+                        if (ok) issue(is_v, j, smem_u32(smem) + S::kRawAt + (uint32_t)to * (kTcStep * D), &sm.raw_full[to]);
+                    }
+                    return li < loads && j < seg.steps;
+                };
+                // loads that exist, in order: the raw ring counts those alone
+                int ahead = 0, to = raw;
+                auto step_ahead = [&]() {
+                    while (ahead < loads && !issue_raw(ahead, to)) ++ahead;
+                    if (ahead < loads) { ++ahead; to = to + 1 == kTcRawSlots ? 0 : to + 1; }
+                };
+                step_ahead();
+                step_ahead();
+                step_ahead();
+                for (int li = 0; li < loads && ok; ++li) {
+                    bool is_v;
+                    int j;
+                    decode(li, is_v, j);
+                    if (j >= seg.steps) continue;
+                    const int t0 = t_first + j * kTcStep;
+                    const bool drafted = t0 + kTcStep > seg.ctx;
+                    // scales of step j: the K load carries those of K and V
+                    float ks[4], vs[4];
+                    const bool scales = !is_v && pw == kTcProducers - 1;
+                    if (scales) {
+#pragma unroll
+                        for (int q = 0; q < 4; ++q) {
+                            const int t = t0 + 32 * q + lane;
+                            const int r = t < total ? tree_pool_row(p, table, t) : -1;
+                            ks[q] = r < 0 ? 0.f : __ldg(p.k_scales + (size_t)r * p.hkv + seg.kvh);
+                            vs[q] = r < 0 ? 0.f : __ldg(p.v_scales + (size_t)r * p.hkv + seg.kvh);
+                        }
+                    }
+                    if (!tc_wait(&sm.raw_full[raw], (raw_phase >> raw) & 1u, abort_flag) || !wait_slot()) { ok = false; break; }
+                    unsigned char* st = smem + S::kRingAt + (uint32_t)slot * S::kSlot;
+                    const unsigned char* rs = smem + S::kRawAt + raw * (kTcStep * D);
+                    const int there = min(total - t0, kTcStep);
+                    bool odd = false;
+#pragma unroll 2
+                    for (int i = pw * 32 + lane; i < kTcStep * (D / 16); i += kTcProducers * 32) {
+                        const int r = i / (D / 16), pc = i % (D / 16);
+                        uint4 c = *reinterpret_cast<const uint4*>(rs + i * 16);
+                        if (drafted && r >= there) c = make_uint4(0, 0, 0, 0);
+                        uint4 a, b;
+                        tree_widen<KV>(c.x, a.x, a.y);
+                        tree_widen<KV>(c.y, a.z, a.w);
+                        tree_widen<KV>(c.z, b.x, b.y);
+                        tree_widen<KV>(c.w, b.z, b.w);
+                        if (KV == kTreeFp8 && is_v && drafted && (tree_odd_chunk(a) || tree_odd_chunk(b))) {
+                            odd = true;
+                            tc_clear_odd(a);
+                            tc_clear_odd(b);
+                        }
+                        unsigned char* row = st + (pc >> 2) * kTcHalf + r * 128;
+                        const int ch = (2 * pc) & 7;
+                        *reinterpret_cast<uint4*>(row + ((ch ^ (r & 7)) << 4)) = a;
+                        *reinterpret_cast<uint4*>(row + (((ch + 1) ^ (r & 7)) << 4)) = b;
+                    }
+                    if (scales) {
+                        const int e = (k_steps + j) & 3;
+                        float top = 0.f;
+#pragma unroll
+                        for (int q = 0; q < 4; ++q) {
+                            // a V scale that is not finite reaches the rows that see its token as its values do
+                            if (!(vs[q] <= 3.402823466e+38f) && drafted) { odd = true; vs[q] = 0.f; }
+                            sc.k[e][32 * q + lane] = ks[q];
+                            sc.v[e][32 * q + lane] = vs[q];
+                            if (vs[q] <= 3.402823466e+38f) top = fmaxf(top, vs[q]);
+                        }
+                        top = warp_max(top);
+                        int ex = -100;
+                        if (top > 0.f) (void)frexpf(top, &ex);
+                        if (lane == 0) sc.v_exp[e] = max(ex, -100);
+                    }
+                    if (odd) sm.odd[(k_steps + j) & 7] = k_steps + j + 1;
+                    asm volatile("fence.proxy.async.shared::cta;\n" ::: "memory");
+                    __syncwarp();
+                    if (lane == 0) { mbar_arrive(&sm.full[slot]); mbar_arrive(&sm.raw_empty[raw]); }
+                    advance();
+                    raw_phase ^= 1u << raw;
+                    raw = raw + 1 == kTcRawSlots ? 0 : raw + 1;
+                    step_ahead();
+                }
+            }
+            k_steps += seg.steps;
+        }
+        if (!ok) { *abort_flag = 1; atomicOr(pp.timeout, 1); }
+    } else {
+        // ============================ tensor cores =========================
+        if (lane == 0) {
+            constexpr uint32_t idesc_s = (1u << 4) | ((uint32_t)(kTcStep >> 3) << 17) | ((128u >> 4) << 24);
+            constexpr uint32_t idesc_o = (1u << 4) | (1u << 16) | ((uint32_t)(D >> 3) << 17) | ((128u >> 4) << 24);
+            const uint32_t q_base = smem_u32(smem), ring = q_base + S::kRingAt;
+            int slot = 0;
+            uint32_t phase = 0;
+            uint32_t q_phase = 0, p_phase[2] = {0, 0};
+            auto take = [&](int& s) -> bool {   // next tile of the ring
+                if (!tc_wait_one(&sm.full[slot], phase, abort_flag)) return false;
+                s = slot;
+                if (++slot == NS) { slot = 0; phase ^= 1u; }
+                return true;
+            };
+            // addresses >> 4: a tile's second half of 64 dims, a step of 16 dims, 16 tokens
+            constexpr uint32_t HALF = kTcHalf >> 4, DIMS = 32u >> 4, TOKENS = 2048u >> 4;
+            auto issue_s = [&](int w, int s) {
+                tc_fence_after();
+                const uint32_t kb = ((ring + (uint32_t)s * S::kSlot) >> 4) | kTcLeadK;
+                const uint32_t qa = ((q_base + (TILES == 2 ? w * QS : 0) * S::kSlot) >> 4) | kTcLeadK;
+                const uint32_t d = tmem + 128u * w;
+#pragma unroll 1
+                for (int q = 0; q < QS; ++q)
+#pragma unroll
+                    for (int kk = 0; kk < D / 16; ++kk) {
+                        const uint32_t in = (uint32_t)(kk >> 2) * HALF + (uint32_t)(kk & 3) * DIMS;
+                        tc_mma_ss(d, qa + (uint32_t)q * (S::kSlot >> 4) + in, kb + in, idesc_s, q || kk);
+                    }
+            };
+            auto issue_o = [&](int w, int s) {
+                const uint32_t vb = ((ring + (uint32_t)s * S::kSlot) >> 4) | kTcLeadV;
+                const uint32_t a = tmem + 128u * w, d = tmem + 256u + 128u * w;
+#pragma unroll 2
+                for (int kk = 0; kk < kTcStep / 16; ++kk)
+#pragma unroll
+                    for (int q = 0; q < QS; ++q)
+                        tc_mma_ts(d, a + 8u * (QS * kk + q), vb + (uint32_t)kk * TOKENS, idesc_o, kk || q);
+            };
+            auto wait_p = [&](int w) -> bool {
+                if (!tc_wait_one(&sm.p_full[w], p_phase[w], abort_flag)) return false;
+                p_phase[w] ^= 1u;
+                tc_fence_after();
+                return true;
+            };
+            while (ok && walk.next(p, seg)) {
+                if (!tc_wait_one(&sm.q_full, q_phase, abort_flag)) { ok = false; break; }
+                q_phase ^= 1u;
+                int ks = 0, vs = 0;
+                if (TILES == 2) {
+                    if (!take(ks)) { ok = false; break; }
+                    issue_s(0, ks);
+                    umma_commit(&sm.s_full[0]);
+                    issue_s(1, ks);
+                    umma_commit(&sm.s_full[1]);
+                    umma_commit(&sm.empty[ks]);
+                    for (int j = 0; j < seg.steps && ok; ++j)
+                        for (int w = 0; w < 2; ++w) {
+                            if (!wait_p(w) || (w == 0 && !take(vs))) { ok = false; break; }
+                            issue_o(w, vs);
+                            if (w == 1) umma_commit(&sm.empty[vs]);
+                            if (j + 1 < seg.steps) {
+                                if (w == 0 && !take(ks)) { ok = false; break; }
+                                issue_s(w, ks);
+                            }
+                            umma_commit(&sm.s_full[w]);
+                            if (w == 1 && j + 1 < seg.steps) umma_commit(&sm.empty[ks]);
+                        }
+                } else {
+                    for (int w = 0; w < 2 && w < seg.steps && ok; ++w) {
+                        if (!take(ks)) { ok = false; break; }
+                        issue_s(w, ks);
+                        umma_commit(&sm.s_full[w]);
+                        umma_commit(&sm.empty[ks]);
+                    }
+                    for (int j = 0; j < seg.steps && ok; ++j) {
+                        const int w = j & 1;
+                        if (!wait_p(w) || !take(vs)) { ok = false; break; }
+                        issue_o(w, vs);
+                        umma_commit(&sm.empty[vs]);
+                        if (j + 2 < seg.steps) {
+                            if (!take(ks)) { ok = false; break; }
+                            issue_s(w, ks);
+                            umma_commit(&sm.empty[ks]);
+                        }
+                        umma_commit(&sm.s_full[w]);
+                    }
+                }
+            }
+            if (!ok) { *abort_flag = 1; atomicOr(pp.timeout, 1); }
+            // every product completes before tensor memory is released
+            umma_commit(&sm.drain);
+            volatile int never = 0;
+            (void)tc_wait_one(&sm.drain, 0u, &never);
+        }
+        __syncwarp();
+    }
+    } else {
+        // ============================ softmax ==============================
+        tc_regs_inc<S::kSoftmaxRegs>();
+        const int w = warp >> 2, quad = warp & 3, row = 32 * quad + lane;
+        const uint32_t lanes = (uint32_t)(32 * quad) << 16;
+        const uint32_t s_addr = tmem + lanes + 128u * w, o_addr = tmem + lanes + 256u + 128u * w;
+        uint32_t q_phase = 0, s_phase = 0, pair_phase = 0, staged_phase = 0;
+        int k_steps = 0;
+        while (ok && walk.next(p, seg)) {
+            const int rows = seg.drafted * p.group;
+            // ---- q rows of the segment's tile: power-of-two scale, fp16 parts; eight lanes a row, each with every
+            //      eighth group of four values ----
+            {
+                constexpr int G = D / 32, B = 2;                    // groups a lane; rows with loads in flight
+                constexpr int NW = TILES == 2 ? 4 : 8;              // warps that share a tile's rows
+                const int tile = TILES == 2 ? w : 0, mine = TILES == 2 ? quad : warp;
+                unsigned char* qt = smem + tile * QS * S::kSlot;
+                const float sign = p.scale < 0.f ? -1.f : 1.f;      // a row's multiplier is not negative
+                const int l8 = lane & 7;
+#pragma unroll 1
+                for (int r0 = mine * 4 + (lane >> 3); r0 < 128; r0 += NW * 4 * B) {
+                    float q[B][4 * G];
+#pragma unroll
+                    for (int x = 0; x < B; ++x) {
+                        const int pr = seg.rt * RT + tile * 128 + r0 + NW * 4 * x;
+                        const bool there = pr < rows;
+                        const int i = there ? pr / p.group : 0;
+                        const size_t at = (size_t)(seg.row0 + i) * p.q_stride + (size_t)(seg.kvh * p.group + (there ? pr - i * p.group : 0)) * p.d;
+#pragma unroll
+                        for (int g = 0; g < G; ++g) {
+                            float v[4] = {0.f, 0.f, 0.f, 0.f};
+                            const int e = 4 * (l8 + 8 * g);
+                            if (there && e < p.d) tree_load<4>(p.q, p.q_type, at + e, v);
+#pragma unroll
+                            for (int k = 0; k < 4; ++k) q[x][4 * g + k] = v[k] * sign;
+                        }
+                    }
+#pragma unroll
+                    for (int x = 0; x < B; ++x) {
+                        const int r = r0 + NW * 4 * x;
+                        float mul = 1.0f;
+                        if (p.q_type != VSPEC_B200_T_F16) {
+                            float top = 0.f;
+#pragma unroll
+                            for (int e = 0; e < 4 * G; ++e) top = fmaxf(top, fabsf(q[x][e]));
+#pragma unroll
+                            for (int o = 4; o > 0; o >>= 1) top = fmaxf(top, __shfl_xor_sync(0xffffffffu, top, o));
+                            // 2^ex with the row's largest value in [2^13, 2^14), as far as normal numbers reach
+                            int ex = (int)(__float_as_uint(top) >> 23) - 126 - 14;
+                            ex = top > 0.f && top <= 3.402823466e+38f ? max(-100, min(100, ex)) : 0;
+                            mul = __uint_as_float((uint32_t)(127 + ex) << 23);
+                            const float inv = __uint_as_float((uint32_t)(127 - ex) << 23);
+#pragma unroll
+                            for (int e = 0; e < 4 * G; ++e) q[x][e] *= inv;
+                        }
+                        // a scale of 0: scores of 0 from products of any size, and -inf stays -inf
+                        if (l8 == 0) sm.mul[tile * 128 + r] = fmaxf(mul * fabsf(p.scale) * kTreeLog2e, 1e-38f);
+#pragma unroll
+                        for (int g = 0; g < G; ++g) {
+                            const int el = 4 * (l8 + 8 * g), ch = el >> 3;
+                            unsigned char* at = qt + (ch >> 3) * kTcHalf + r * 128 + (((ch & 7) ^ (r & 7)) << 4) + (el & 4) * 2;
+                            float* v = &q[x][4 * g];
+#pragma unroll
+                            for (int s = 0; s < QS; ++s) {
+                                const uint32_t h0 = tree_pack(v[0], v[1]), h1 = tree_pack(v[2], v[3]);
+                                const float2 u0 = tree_unpack(h0), u1 = tree_unpack(h1);
+                                v[0] -= u0.x; v[1] -= u0.y; v[2] -= u1.x; v[3] -= u1.y;
+                                *reinterpret_cast<uint2*>(at + s * S::kSlot) = make_uint2(h0, h1);
+                            }
+                        }
+                    }
+                }
+                asm volatile("fence.proxy.async.shared::cta;\n" ::: "memory");
+                mbar_arrive(&sm.q_full);
+                if (!tc_wait(&sm.q_full, q_phase, abort_flag)) { ok = false; break; }
+                q_phase ^= 1u;
+            }
+            const int local = (TILES == 2 ? 128 * w : 0) + row;     // row of the tile pair
+            const int pr = seg.rt * RT + local;
+            const bool in = pr < rows;
+            const int ti = in ? pr / p.group : 0;
+            const float mul = sm.mul[local];
+            float o[D];
+#pragma unroll
+            for (int i = 0; i < D; ++i) o[i] = 0.f;
+            float m = kTreeLowest, l = 0.f, f = 1.f;
+            int v_exp = -100, prev_j = -1;
+            // the product of the step before: o = o f + P V
+            auto add_o = [&]() {
+                const int tag = k_steps + prev_j + 1;
+                tc_sweep<D / 16>(o_addr, [&](int c, float (&v)[16]) {
+#pragma unroll
+                    for (int i = 0; i < 16; ++i) o[16 * c + i] = fmaf(o[16 * c + i], f, v[i]);
+                });
+                if (sm.odd[(tag - 1) & 7] == tag) {
+                    // infinities and NaN among the step's drafted tokens, for the rows that see them
+                    const int32_t* table = p.table + (size_t)seg.b * p.max_pages;
+                    const int t0 = (seg.step0 + prev_j) * kTcStep;
+                    for (int t = max(t0, seg.ctx); t < min(t0 + kTcStep, seg.ctx + seg.drafted); ++t) {
+                        if (!in || !tree_sees(p, seg.row0, ti, seg.ctx, seg.drafted, t)) continue;
+                        const size_t head = (size_t)tree_pool_row(p, table, t) * p.hkv + seg.kvh, at = head * p.d;
+                        const float vs = KV == kTreeF16 ? 1.f : __ldg(p.v_scales + head);
+#pragma unroll
+                        for (int i = 0; i < D; ++i) {
+                            if (i >= p.d) continue;
+                            float v;
+                            if (KV == kTreeF16) {
+                                v = __half2float(reinterpret_cast<const __half*>(p.v_pages)[at + i]);
+                            } else {
+                                const uint8_t code = reinterpret_cast<const uint8_t*>(p.v_pages)[at + i];
+                                v = KV == kTreeFp8 ? __half2float(__half(__nv_cvt_fp8_to_halfraw(code, __NV_E4M3))) : (float)(int8_t)code;
+                                v *= vs;
+                            }
+                            if (!isfinite(v)) o[i] += v;
+                        }
+                    }
+                }
+            };
+            const int n = TILES == 2 ? seg.steps : (seg.steps - w + 1) / 2;
+            // one pass more than steps: it adds the last step's product
+            for (int i = 0; i <= n && n > 0; ++i) {
+                const int j = TILES == 2 ? i : 2 * i + w;
+                if (!tc_wait(&sm.s_full[w], s_phase, abort_flag)) { ok = false; break; }
+                s_phase ^= 1u;
+                tc_fence_after();
+                if (i > 0) add_o();
+                if (i == n) break;
+                prev_j = j;
+                const int t0 = (seg.step0 + j) * kTcStep, e4 = (k_steps + j) & 3;
+                const bool masked = t0 + kTcStep > seg.ctx;
+                const float* ks = KV == kTreeF16 ? nullptr : sc.k[e4];
+                if (masked) {
+                    // what the row does not see becomes -inf in S; the scales of K are applied on the way
+#pragma unroll 1
+                    for (int c = 0; c < 8; ++c) {
+                        float v[16];
+                        tmem_ld_x16(s_addr + 16u * c, v);
+                        const uint32_t see = in ? tc_sees32(p, seg.row0, ti, seg.drafted, t0 + 16 * c - seg.ctx) : 0u;
+                        tc_landed(v);
+                        uint32_t h[16];
+#pragma unroll
+                        for (int x = 0; x < 16; ++x) {
+                            if (KV != kTreeF16) v[x] *= ks[16 * c + x];
+                            h[x] = (see >> x) & 1u ? __float_as_uint(v[x]) : 0xFF800000u;
+                        }
+                        tc_st_x16(s_addr + 16u * c, h);
+                    }
+                    tmem_wait_st();
+                    ks = sc.one;
+                }
+                // ---- maximum ----
+                float tops[2] = {-INFINITY, -INFINITY};
+                tc_sweep<8>(s_addr, [&](int c, float (&v)[16]) {
+                    tc_scale<KV != kTreeF16>(v, ks + 16 * c);
+#pragma unroll
+                    for (int x = 0; x < 16; ++x) tops[x & 1] = fmaxf(tops[x & 1], v[x]);
+                });
+                const float top = fmaxf(tops[0], tops[1]);
+                const float m_new = top == -INFINITY ? m : fmaxf(m, top * mul);
+                f = tree_ex2(m - m_new);
+                m = m_new;
+                if (KV != kTreeF16) {
+                    const int ex = sc.v_exp[e4];
+                    if (ex > v_exp) {
+                        f *= v_exp > -100 ? ldexpf(1.0f, max(v_exp - ex, -126)) : 0.f;
+                        v_exp = ex;
+                    }
+                }
+                // ---- weights 2^(s - m + 14 - v_exp), over S: 16 tokens at a time ----
+                const float bias = (KV == kTreeF16 ? 14.f : (float)(14 - v_exp)) - m_new;
+                float ls[4] = {0.f, 0.f, 0.f, 0.f};
+                tc_sweep<8>(s_addr, [&](int c, float (&v)[16]) {
+                    tc_scale<KV != kTreeF16>(v, ks + 16 * c);
+#pragma unroll
+                    for (int x = 0; x < 16; ++x) v[x] = tree_ex2(fmaf(v[x], mul, bias));
+#pragma unroll
+                    for (int x = 0; x < 16; ++x) ls[x & 3] += v[x];
+                    tc_scale<KV != kTreeF16>(v, &sc.v[e4][16 * c]);
+                    uint32_t h[8];
+#pragma unroll
+                    for (int x = 0; x < 8; ++x) h[x] = tree_pack(v[2 * x], v[2 * x + 1]);
+                    if constexpr (QS == 2) {
+                        // 8 columns of high parts, 8 of low parts
+                        tc_st_x8(s_addr + 16u * c, h);
+#pragma unroll
+                        for (int x = 0; x < 8; ++x) {
+                            const float2 u = tree_unpack(h[x]);
+                            h[x] = tree_pack(v[2 * x] - u.x, v[2 * x + 1] - u.y);
+                        }
+                        tc_st_x8(s_addr + 16u * c + 8u, h);
+                    } else {
+                        tc_st_x8(s_addr + 8u * c, h);
+                    }
+                });
+                l = fmaf(l, f, (ls[0] + ls[1]) + (ls[2] + ls[3]));
+                tmem_wait_st();
+                tc_fence_before();
+                mbar_arrive(&sm.p_full[w]);
+            }
+            if (!ok) break;
+            k_steps += seg.steps;
+            // ---- the rows: natural scale, the two groups' halves joined, out ----
+            const float unit = ldexpf(1.0f / kTreePScale, KV == kTreeF16 ? 0 : v_exp);
+            l *= unit;
+#pragma unroll
+            for (int i = 0; i < D; ++i) o[i] *= unit;
+            if (TILES == 1) {
+                if (w == 1) {
+                    sm.ml[0][row] = m;
+                    sm.ml[1][row] = l;
+#pragma unroll
+                    for (int c = 0; c < D / 32; ++c) {
+                        uint32_t h[32];
+#pragma unroll
+                        for (int i = 0; i < 32; ++i) h[i] = __float_as_uint(o[32 * c + i]);
+                        tmem_st_x32(o_addr + 32u * c, h);
+                    }
+                    tmem_wait_st();
+                }
+                tc_fence_before();
+                mbar_arrive(&sm.pair);
+                if (!tc_wait(&sm.pair, pair_phase, abort_flag)) { ok = false; break; }
+                pair_phase ^= 1u;
+                tc_fence_after();
+                if (w == 0) {
+                    const float m1 = sm.ml[0][row], l1 = sm.ml[1][row];
+                    const float M = fmaxf(m, m1), f0 = tree_ex2(m - M), f1 = tree_ex2(m1 - M);
+                    m = M;
+                    l = l * f0 + l1 * f1;
+                    tc_sweep<D / 16>(o_addr + 128u, [&](int c, float (&v)[16]) {
+#pragma unroll
+                        for (int i = 0; i < 16; ++i) o[16 * c + i] = o[16 * c + i] * f0 + v[i] * f1;
+                    });
+                }
+                tc_fence_before();           // the wait below: the second group's O and (m, l) have been read
+            }
+            if (TILES == 2 || w == 0) {
+                // rows out through this warp's quarter of the q tile, whose products are done, CW values of each at a
+                // time: a lane puts its row in, then lanes side by side store pieces of one row
+                constexpr int CW = QS * D / 2 < 64 ? QS * D / 2 : 64, LPR = CW / 4;
+                const bool whole = seg.steps == seg.n;
+                const float inv = !whole ? 1.f : (l == 0.f ? 0.f : 1.0f / l);
+                float4* stage = reinterpret_cast<float4*>(smem + (TILES == 2 ? w * QS : 0) * S::kSlot + quad * (32 * CW * 4));
+#pragma unroll
+                for (int c = 0; c < D / CW; ++c) {
+                    __syncwarp();
+#pragma unroll
+                    for (int i = 0; i < LPR; ++i) {
+                        const float* v = o + CW * c + 4 * i;
+                        stage[lane * LPR + (i ^ (lane & 7))] = whole && l == 0.f ? make_float4(0.f, 0.f, 0.f, 0.f)
+                            : make_float4(v[0] * inv, v[1] * inv, v[2] * inv, v[3] * inv);
+                    }
+                    __syncwarp();
+                    const int piece = lane % LPR, e = CW * c + 4 * piece;
+#pragma unroll 4
+                    for (int i = 0; i < 32; i += 32 / LPR) {
+                        const int r = i + lane / LPR, lr = (TILES == 2 ? 128 * w : 0) + 32 * quad + r, pr2 = seg.rt * RT + lr;
+                        const float4 v = stage[r * LPR + (piece ^ (r & 7))];
+                        if (pr2 < rows && e < p.d) {
+                            if (whole) {
+                                const int i2 = pr2 / p.group;
+                                tree_store4(p.out, p.q_type, ((size_t)(seg.row0 + i2) * p.hq + (size_t)seg.kvh * p.group + pr2 - i2 * p.group) * p.d + e, v, 1.f, false);
+                            } else {
+                                *reinterpret_cast<float4*>(p.part_o + ((size_t)(2 * blockIdx.x + (seg.step0 == 0 ? 1 : 0)) * RT + lr) * p.d + e) = v;
+                            }
+                        }
+                    }
+                }
+                if (!whole && in)
+                    *reinterpret_cast<float2*>(p.part_ml + ((size_t)(2 * blockIdx.x + (seg.step0 == 0 ? 1 : 0)) * RT + local) * 2) = make_float2(m, l);
+            }
+            // every warp's stage has been read before any writes the next segment's q there
+            uint64_t* read = TILES == 1 ? &sm.pair : &sm.staged[w];
+            mbar_arrive(read);
+            if (!tc_wait(read, TILES == 1 ? pair_phase : staged_phase, abort_flag)) { ok = false; break; }
+            if (TILES == 1) pair_phase ^= 1u; else staged_phase ^= 1u;
+            tc_fence_after();
+        }
+        if (!ok) { *abort_flag = 1; atomicOr(pp.timeout, 1); }
+    }
+    tc_fence_before();
+    __syncthreads();
+    tc_fence_after();
+    if (warp == kTcMmaWarp) tmem_dealloc(tmem, 512);
+}
+
+// Joins the parts of the pairs that were cut.  Block column x stands for the cut
+// between CTAs x and x + 1; the first cut within a pair joins all its parts, in
+// order: the first is in the second part slot of its CTA, the others in the
+// first of theirs.  Eight warps of a block take rows in turn.
+template <int RT>
+__global__ void __launch_bounds__(256) tree_tc_combine_kernel(const TreeParams p) {
+    pdl_wait();
+    pdl_trigger();
+    const int lane = threadIdx.x & 31, warp = threadIdx.x >> 5, most = gridDim.x + 1, cut = blockIdx.x + 1;
+    long long total = 0;
+    for (int b0 = 0; b0 < p.batch; b0 += 32) {
+        int n, tiles;
+        long long w = b0 + lane < p.batch ? tc_work<RT>(p, b0 + lane, n, tiles) : 0;
+#pragma unroll
+        for (int o = 16; o > 0; o >>= 1) w += __shfl_xor_sync(0xffffffffu, w, o);
+        total += w;
+    }
+    const int g = tc_ctas(total, most);
+    if (cut >= g) return;
+    const long long at = total * cut / g;      // first step behind the cut
+    // its sequence
+    long long before = 0;
+    int b = -1;
+    for (int b0 = 0; b0 < p.batch && b < 0; b0 += 32) {
+        int n, tiles;
+        const long long w = b0 + lane < p.batch ? tc_work<RT>(p, b0 + lane, n, tiles) : 0;
+        long long incl = w;
+#pragma unroll
+        for (int o = 1; o < 32; o <<= 1) {
+            const long long u = __shfl_up_sync(0xffffffffu, incl, o);
+            if (lane >= o) incl += u;
+        }
+        const unsigned hit = __ballot_sync(0xffffffffu, before + incl > at);
+        if (hit) {
+            const int x = __ffs(hit) - 1;
+            b = b0 + x;
+            before += __shfl_sync(0xffffffffu, incl - w, x);
+        } else {
+            before += __shfl_sync(0xffffffffu, incl, 31);
+        }
+    }
+    int n, tiles, row0;
+    (void)tc_work<RT>(p, b, n, tiles);
+    const int drafted = tree_rows(p, b, row0), rows = drafted * p.group;
+    const int pair = (int)((at - before) / n);
+    const long long start = before + (long long)pair * n;
+    if (start == at) return;                   // between two pairs
+    // the CTA of step s: the largest c with total c / g <= s
+    const int first = (int)(((start + 1) * g + total - 1) / total) - 1;
+    const int last = (int)(((start + n) * g + total - 1) / total) - 1;
+    if (first != cut - 1) return;              // not the pair's first cut
+    const int kvh = pair / tiles, rt = pair - kvh * tiles;
+    const float2* ml = reinterpret_cast<const float2*>(p.part_ml);
+    const int e = lane * 4;
+    for (int local = blockIdx.y * 8 + warp; local < RT; local += gridDim.y * 8) {
+        const int pr = rt * RT + local;
+        if (pr >= rows) return;
+        auto slot = [&](int c) { return (size_t)(2 * c + (c == first ? 1 : 0)) * RT + local; };
+        float M = kTreeLowest;
+        for (int c = first; c <= last; ++c) M = fmaxf(M, ml[slot(c)].x);
+        float L = 0.f;
+        float4 acc = {0.f, 0.f, 0.f, 0.f};
+#pragma unroll 4
+        for (int c = first; c <= last; ++c) {
+            const float2 x = ml[slot(c)];
+            const float w = tree_ex2(x.x - M);
+            L += x.y * w;
+            if (e < p.d) {
+                const float4 v = *reinterpret_cast<const float4*>(p.part_o + slot(c) * p.d + e);
+                acc.x += v.x * w; acc.y += v.y * w; acc.z += v.z * w; acc.w += v.w * w;
+            }
+        }
+        const int i = pr / p.group;
+        const size_t orow = (size_t)(row0 + i) * p.hq + (size_t)kvh * p.group + (pr - i * p.group);
+        if (e < p.d) tree_store4(p.out, p.q_type, orow * p.d + e, acc, L == 0.f ? 0.f : 1.0f / L, L == 0.f);
+    }
+}
+
+template <int D, int TILES, int QS, int KV>
+cudaError_t tree_tc_launch_one(const TcParams& pp, int ctas, cudaStream_t st) {
+    static int configured[64] = {0};
+    int dev = 0;
+    cudaError_t e = cudaGetDevice(&dev);
+    if (e != cudaSuccess) return e;
+    constexpr uint32_t bytes = TcShape<D, TILES, QS, KV>::kTotal;
+    if (dev < 0 || dev >= 64 || !configured[dev]) {
+        e = cudaFuncSetAttribute(tree_tc_kernel<D, TILES, QS, KV>, cudaFuncAttributeMaxDynamicSharedMemorySize, (int)bytes);
+        if (e != cudaSuccess) return e;
+        if (dev >= 0 && dev < 64) configured[dev] = 1;
+    }
+    e = launch_pdl(tree_tc_kernel<D, TILES, QS, KV>, dim3(ctas), dim3(TcShape<D, TILES, QS, KV>::kThreads), bytes, st, pp);
+    if (e != cudaSuccess) return e;
+    if (ctas == 1) return cudaSuccess;
+    return launch_pdl(tree_tc_combine_kernel<128 * TILES>, dim3(ctas - 1, 4), dim3(256), 0, st, pp.t);
+}
+
+// Row tiles a CTA: two for pairs of more than 128 rows; 8-bit pages with fp32 q
+// have no room for the two tiles' parts beside the raw ring.
+inline int tree_tc_tiles(int rows, bool f16_pages, int q_type) {
+    return rows > 128 && (f16_pages || q_type != VSPEC_B200_T_F32) ? 2 : 1;
+}
+
+template <int D, int KV>
+cudaError_t tree_tc_pick(const TcParams& pp, int ctas, cudaStream_t st) {
+    const bool two = pp.t.q_type == VSPEC_B200_T_F32;
+    const int tiles = tree_tc_tiles(pp.t.max_q * pp.t.group, KV == kTreeF16, pp.t.q_type);
+    if (tiles == 1) return two ? tree_tc_launch_one<D, 1, 2, KV>(pp, ctas, st) : tree_tc_launch_one<D, 1, 1, KV>(pp, ctas, st);
+    if constexpr (KV == kTreeF16)
+        if (two) return tree_tc_launch_one<D, 2, 2, KV>(pp, ctas, st);
+    return tree_tc_launch_one<D, 2, 1, KV>(pp, ctas, st);
+}
+
+// Boxes of box_rows pool rows x one KV head x 64 fp16 values or a whole row of D codes.
+inline int tree_tc_map(CUtensorMap* map, const void* pages, const TreeParams& p, bool f16, int box_rows) {
+    PFN_cuTensorMapEncodeTiled_v12000 enc = tensor_map_encoder();
+    if (!enc) { set_error("cuTensorMapEncodeTiled unavailable"); return VSPEC_B200_ERR_CUDA; }
+    const cuuint64_t es = f16 ? 2 : 1;
+    cuuint64_t dims[3] = {(cuuint64_t)p.d, (cuuint64_t)p.hkv, (cuuint64_t)p.num_pages * (cuuint64_t)p.page_tokens};
+    cuuint64_t strides[2] = {(cuuint64_t)p.d * es, (cuuint64_t)p.hkv * p.d * es};
+    cuuint32_t box[3] = {f16 ? 64u : (p.d <= 64 ? 64u : 128u), 1u, (cuuint32_t)box_rows};
+    cuuint32_t estr[3] = {1, 1, 1};
+    const CUresult r = enc(map, f16 ? CU_TENSOR_MAP_DATA_TYPE_FLOAT16 : CU_TENSOR_MAP_DATA_TYPE_UINT8, 3,
+                           const_cast<void*>(pages), dims, strides, box, estr, CU_TENSOR_MAP_INTERLEAVE_NONE,
+                           f16 ? CU_TENSOR_MAP_SWIZZLE_128B : CU_TENSOR_MAP_SWIZZLE_NONE,
+                           CU_TENSOR_MAP_L2_PROMOTION_L2_256B, CU_TENSOR_MAP_FLOAT_OOB_FILL_NONE);
+    if (r != CUDA_SUCCESS) { set_error("cuTensorMapEncodeTiled failed (%d)", (int)r); return VSPEC_B200_ERR_CUDA; }
+    return VSPEC_B200_OK;
+}
+
+template <int KV>
+cudaError_t tree_tc_launch(const TcParams& pp, int ctas, cudaStream_t st) {
+    return pp.t.d <= 64 ? tree_tc_pick<64, KV>(pp, ctas, st) : tree_tc_pick<128, KV>(pp, ctas, st);
+}
+
+// one translation unit per page type
+extern template cudaError_t tree_tc_launch<kTreeF16>(const TcParams&, int, cudaStream_t);
+extern template cudaError_t tree_tc_launch<kTreeFp8>(const TcParams&, int, cudaStream_t);
+extern template cudaError_t tree_tc_launch<kTreeInt8>(const TcParams&, int, cudaStream_t);
+
+}  // namespace vb200

@@ -212,6 +212,7 @@ _sigs = {
     "vspec_b200_kv_quant_gather": ([POINTER(KvGatherArgs), c_void_p], c_int),
     "vspec_b200_tree_attention_workspace_bytes": ([c_size_t] * 7, c_size_t),
     "vspec_b200_tree_attention": ([POINTER(TreeAttnArgs), c_void_p], c_int),
+    "vspec_b200_tree_attention_timeout_flag": ([POINTER(c_int)], c_int),
     "vspec_b200_logprobs_workspace_bytes": ([c_size_t] * 3, c_size_t),
     "vspec_b200_logprobs": ([POINTER(LogprobsArgs), c_void_p], c_int),
     "vspec_b200_rmsnorm_f32": ([c_void_p, c_void_p, c_float, c_size_t, c_size_t, c_void_p, c_void_p], c_int),
@@ -418,6 +419,12 @@ def tree_attention(q: int, k_pages: int, v_pages: int, k_scales: int | None, v_s
                      max_q, hq, hkv, d, page_tokens, max_pages, num_pages, max_ctx, mask_words, q_stride, scale,
                      q_dtype, kv_dtype, workspace, workspace_bytes)
     check(lib.vspec_b200_tree_attention(ctypes.byref(a), stream), "vspec_b200_tree_attention")
+
+
+def tree_attention_timeout_flag() -> int:
+    v = c_int(0)
+    check(lib.vspec_b200_tree_attention_timeout_flag(ctypes.byref(v)), "tree_attention_timeout_flag")
+    return v.value
 
 
 def logprobs(logits: int, rows: int, vocab: int, dtype: int = T_F32, tokens: int | None = None, num_tokens: int = 0,
