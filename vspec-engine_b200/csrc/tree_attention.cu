@@ -92,9 +92,9 @@ static TreePlan tree_plan(size_t batch, size_t max_q, size_t hq, size_t hkv, siz
     const long long rows = (long long)max_q * (long long)(hq / hkv);
     t.tc = tree_uses_tc(rows, d, page_tokens);
     if (t.tc) {
-        const long long steps = (long long)batch * hkv * ((rows + 127) / 128) * (((long long)max_ctx + kTcStep - 1) / kTcStep);
+        const long long units = (long long)batch * hkv * ((rows + 127) / 128) * (((long long)max_ctx + kTcStep - 1) / kTcStep + kTcPairCost);
         const long long most = device_sm_count();
-        t.ctas = (int)((steps + 1) / 2 < most ? (steps + 1) / 2 : most);
+        t.ctas = (int)((units + 2) / 3 < most ? (units + 2) / 3 : most);
         t.max_splits = 1;
         return t;
     }

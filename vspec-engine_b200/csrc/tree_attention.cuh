@@ -49,27 +49,32 @@ __device__ __forceinline__ int tree_rows(const TreeParams& p, int b, int& row0) 
     return row0 < 0 || row0 >= end ? 0 : min(end - row0, p.max_q);
 }
 
-// N (2, 4 or 8) consecutive values of q from element i on (i a multiple of N).
-template <int N>
-__device__ __forceinline__ void tree_load(const void* p, int type, size_t i, float (&v)[N]) {
-    if (type == VSPEC_B200_T_F32) {
-        constexpr int M = N < 4 ? N : 4;
+// N (2, 4 or 8) consecutive values of q from each of R places (multiples of N), 0
+// where at[r] is kTreeNone.  Every load is issued whatever its place, so that all
+// of them are in flight at once: a branch around each made them wait for one
+// another (6300 cycles for eight loads against 900).
+constexpr size_t kTreeNone = ~(size_t)0;
+template <typename T, int N, int R>
+__device__ __forceinline__ void tree_load_as(const void* p, const size_t (&at)[R], float (&v)[R][N]) {
+    constexpr int M = N * sizeof(T) > 16 ? 16 / sizeof(T) : N;
+    Vec<T, M> w[R][N / M];
 #pragma unroll
-        for (int x = 0; x < N; x += M) {
-            const Vec<float, M> w = *reinterpret_cast<const Vec<float, M>*>(reinterpret_cast<const float*>(p) + i + x);
+    for (int r = 0; r < R; ++r)
 #pragma unroll
-            for (int e = 0; e < M; ++e) v[x + e] = w.e[e];
-        }
-    } else if (type == VSPEC_B200_T_F16) {
-        const Vec<__half, N> w = *reinterpret_cast<const Vec<__half, N>*>(reinterpret_cast<const __half*>(p) + i);
+        for (int x = 0; x < N / M; ++x)
+            w[r][x] = *reinterpret_cast<const Vec<T, M>*>(reinterpret_cast<const T*>(p) + (at[r] == kTreeNone ? 0 : at[r]) + x * M);
 #pragma unroll
-        for (int e = 0; e < N; ++e) v[e] = __half2float(w.e[e]);
-    } else {
-        const Vec<__nv_bfloat16, N> w = *reinterpret_cast<const Vec<__nv_bfloat16, N>*>(reinterpret_cast<const __nv_bfloat16*>(p) + i);
+    for (int r = 0; r < R; ++r)
 #pragma unroll
-        for (int e = 0; e < N; ++e) v[e] = __bfloat162float(w.e[e]);
-    }
+        for (int e = 0; e < N; ++e) v[r][e] = at[r] == kTreeNone ? 0.f : elem_to_f32<T>(w[r][e / M].e[e % M]);
 }
+template <int N, int R>
+__device__ __forceinline__ void tree_load(const void* p, int type, const size_t (&at)[R], float (&v)[R][N]) {
+    if (type == VSPEC_B200_T_F32) tree_load_as<float>(p, at, v);
+    else if (type == VSPEC_B200_T_F16) tree_load_as<__half>(p, at, v);
+    else tree_load_as<__nv_bfloat16>(p, at, v);
+}
+
 // Four values v * inv in a row (0 for a row that saw nothing), rounded once.
 __device__ __forceinline__ void tree_store4(void* p, int type, size_t i, float4 v, float inv, bool empty) {
     v = empty ? make_float4(0.f, 0.f, 0.f, 0.f) : make_float4(v.x * inv, v.y * inv, v.z * inv, v.w * inv);

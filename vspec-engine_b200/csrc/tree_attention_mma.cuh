@@ -135,17 +135,15 @@ __global__ void __launch_bounds__(kTreeThreads) tree_mma_kernel(const TreeParams
         float q[B][E];
 #pragma unroll 1
         for (int r0 = warp; r0 < MT; r0 += 4 * B) {
+        size_t at[B];
 #pragma unroll
         for (int x = 0; x < B; ++x) {
             const int pr = rt * MT + r0 + 4 * x;
-            if (pr < rows && lane * E < p.d) {
-                tree_load<E>(p.q, p.q_type, (size_t)(row0 + pr / p.group) * p.q_stride +
-                             (size_t)(kvh * p.group + pr % p.group) * p.d + lane * E, q[x]);
-            } else {
-#pragma unroll
-                for (int e = 0; e < E; ++e) q[x][e] = 0.f;
-            }
+            at[x] = pr < rows && lane * E < p.d ? (size_t)(row0 + pr / p.group) * p.q_stride +
+                                                      (size_t)(kvh * p.group + pr % p.group) * p.d + lane * E
+                                                : kTreeNone;
         }
+        tree_load<E, B>(p.q, p.q_type, at, q);
 #pragma unroll
         for (int x = 0; x < B; ++x) {
             const int r = r0 + 4 * x;

@@ -67,7 +67,7 @@ struct TcShape {
 // misc area
 struct alignas(16) TcMisc {
     float mul[256];             // score multiplier of each row
-    uint64_t full[6], empty[6], raw_full[kTcRawSlots], raw_empty[kTcRawSlots], s_full[2], p_full[2], q_full, pair, staged[2], drain;
+    uint64_t full[6], empty[6], raw_full[kTcRawSlots], raw_empty[kTcRawSlots], s_full[2], p_half[2], p_full[2], q_full, pair, staged[2], drain;
     uint32_t tmem;
     int abort;
     int start_b;
@@ -172,7 +172,9 @@ __device__ __forceinline__ bool tc_wait(uint64_t* bar, uint32_t parity, volatile
     return __all_sync(0xffffffffu, tc_wait_one(bar, parity, abort));
 }
 
-// ---- the work: sequence b has pairs (KV head, row tile) of n steps each ----
+// ---- the work: sequence b has pairs (KV head, row tile) of n steps each.  A pair also costs its q rows, its
+//      output and the filling of the pipeline, about kTcPairCost steps: runs are equal in steps and those ----
+constexpr int kTcPairCost = 2;
 template <int RT>
 __device__ __forceinline__ long long tc_work(const TreeParams& p, int b, int& n, int& tiles) {
     int row0;
@@ -180,11 +182,11 @@ __device__ __forceinline__ long long tc_work(const TreeParams& p, int b, int& n,
     const int total = max(p.ctx_len[b], 0) + drafted;
     n = (total + kTcStep - 1) / kTcStep;
     tiles = (drafted * p.group + RT - 1) / RT;
-    return drafted ? (long long)n * p.hkv * tiles : 0;
+    return drafted ? (long long)(n + kTcPairCost) * p.hkv * tiles : 0;
 }
-// CTAs that take part: at least two steps each.
+// CTAs that take part: at least three units each.
 __device__ __forceinline__ int tc_ctas(long long total, int most) {
-    const long long g = (total + 1) / 2;
+    const long long g = (total + 2) / 3;
     return (int)(g < 1 ? 1 : (g < most ? g : most));
 }
 
@@ -202,17 +204,21 @@ struct TcWalk {
             int n, tiles;
             const long long w = tc_work<RT>(p, b, n, tiles);
             if (off >= w) { off -= w; ++b; continue; }
+            // a pair's units: kTcPairCost, then its steps
+            const int units = n + kTcPairCost;
+            const long long pair = off >> 31 ? off / units : (long long)((unsigned)off / (unsigned)units);
+            const int u0 = (int)(off - pair * units), u1 = (int)min((long long)units, u0 + left);
+            off += u1 - u0;
+            left -= u1 - u0;
+            s.step0 = max(u0 - kTcPairCost, 0);
+            s.steps = max(u1 - kTcPairCost, 0) - s.step0;
+            if (s.steps == 0) continue;        // only the pair's cost: the next CTA begins its first step
             s.b = b;
             s.drafted = tree_rows(p, b, s.row0);
             s.ctx = max(p.ctx_len[b], 0);
             s.n = n;
-            const long long pair = off / n;
-            s.step0 = (int)(off - pair * n);
-            s.kvh = (int)(pair / tiles);
-            s.rt = (int)(pair - (long long)s.kvh * tiles);
-            s.steps = (int)min((long long)(n - s.step0), left);
-            off += s.steps;
-            left -= s.steps;
+            s.kvh = (int)pair / tiles;         // pairs of a sequence: at most 65535
+            s.rt = (int)pair - s.kvh * tiles;
             return true;
         }
         return false;
@@ -265,7 +271,7 @@ __global__ void __launch_bounds__(TcShape<D, TILES, QS, KV>::kThreads, 1) tree_t
         sm.abort = 0;
         for (int i = 0; i < 6; ++i) { mbar_init(&sm.full[i], kTcProducers); mbar_init(&sm.empty[i], 1); }
         for (int i = 0; i < kTcRawSlots; ++i) { mbar_init(&sm.raw_full[i], 1); mbar_init(&sm.raw_empty[i], kTcProducers); }
-        for (int i = 0; i < 2; ++i) { mbar_init(&sm.s_full[i], 1); mbar_init(&sm.p_full[i], 128); }
+        for (int i = 0; i < 2; ++i) { mbar_init(&sm.s_full[i], 1); mbar_init(&sm.p_half[i], 128); mbar_init(&sm.p_full[i], 128); }
         mbar_init(&sm.q_full, 256);
         mbar_init(&sm.pair, 256);
         for (int i = 0; i < 2; ++i) mbar_init(&sm.staged[i], 128);
@@ -556,18 +562,21 @@ __global__ void __launch_bounds__(TcShape<D, TILES, QS, KV>::kThreads, 1) tree_t
                         tc_mma_ss(d, qa + (uint32_t)q * (S::kSlot >> 4) + in, kb + in, idesc_s, q || kk);
                     }
             };
-            auto issue_o = [&](int w, int s) {
+            auto issue_o = [&](int w, int s, int half) {   // over half of the step's tokens
                 const uint32_t vb = ((ring + (uint32_t)s * S::kSlot) >> 4) | kTcLeadV;
                 const uint32_t a = tmem + 128u * w, d = tmem + 256u + 128u * w;
-#pragma unroll 2
-                for (int kk = 0; kk < kTcStep / 16; ++kk)
+#pragma unroll 1
+                for (int k2 = 2 * half; k2 < 2 * half + 2; ++k2)
 #pragma unroll
-                    for (int q = 0; q < QS; ++q)
-                        tc_mma_ts(d, a + 8u * (QS * kk + q), vb + (uint32_t)kk * TOKENS, idesc_o, kk || q);
+                    for (int k1 = 0; k1 < 2; ++k1)
+#pragma unroll
+                        for (int q = 0; q < QS; ++q)
+                            tc_mma_ts(d, a + 8u * (QS * (2 * k2 + k1) + q), vb + (uint32_t)(2 * k2 + k1) * TOKENS, idesc_o, k2 || k1 || q);
             };
-            auto wait_p = [&](int w) -> bool {
-                if (!tc_wait_one(&sm.p_full[w], p_phase[w], abort_flag)) return false;
-                p_phase[w] ^= 1u;
+            // the two halves of a step's weights have a barrier each: one barrier's second completion would hide the first
+            auto wait_p = [&](int w, int half) -> bool {
+                if (!tc_wait_one(half ? &sm.p_full[w] : &sm.p_half[w], p_phase[w], abort_flag)) return false;
+                if (half) p_phase[w] ^= 1u;
                 tc_fence_after();
                 return true;
             };
@@ -584,8 +593,10 @@ __global__ void __launch_bounds__(TcShape<D, TILES, QS, KV>::kThreads, 1) tree_t
                     umma_commit(&sm.empty[ks]);
                     for (int j = 0; j < seg.steps && ok; ++j)
                         for (int w = 0; w < 2; ++w) {
-                            if (!wait_p(w) || (w == 0 && !take(vs))) { ok = false; break; }
-                            issue_o(w, vs);
+                            if ((w == 0 && !take(vs)) || !wait_p(w, 0)) { ok = false; break; }
+                            issue_o(w, vs, 0);
+                            if (!wait_p(w, 1)) { ok = false; break; }
+                            issue_o(w, vs, 1);
                             if (w == 1) umma_commit(&sm.empty[vs]);
                             if (j + 1 < seg.steps) {
                                 if (w == 0 && !take(ks)) { ok = false; break; }
@@ -603,8 +614,10 @@ __global__ void __launch_bounds__(TcShape<D, TILES, QS, KV>::kThreads, 1) tree_t
                     }
                     for (int j = 0; j < seg.steps && ok; ++j) {
                         const int w = j & 1;
-                        if (!wait_p(w) || !take(vs)) { ok = false; break; }
-                        issue_o(w, vs);
+                        if (!take(vs) || !wait_p(w, 0)) { ok = false; break; }
+                        issue_o(w, vs, 0);
+                        if (!wait_p(w, 1)) { ok = false; break; }
+                        issue_o(w, vs, 1);
                         umma_commit(&sm.empty[vs]);
                         if (j + 2 < seg.steps) {
                             if (!take(ks)) { ok = false; break; }
@@ -631,7 +644,9 @@ __global__ void __launch_bounds__(TcShape<D, TILES, QS, KV>::kThreads, 1) tree_t
         const uint32_t s_addr = tmem + lanes + 128u * w, o_addr = tmem + lanes + 256u + 128u * w;
         uint32_t q_phase = 0, s_phase = 0, pair_phase = 0, staged_phase = 0;
         int k_steps = 0;
-        while (ok && walk.next(p, seg)) {
+        TcSegment ahead;
+        bool more = walk.next(p, seg);
+        for (; ok && more; seg = ahead) {
             const int rows = seg.drafted * p.group;
             // ---- q rows of the segment's tile: power-of-two scale, fp16 parts; eight lanes a row, each with every
             //      eighth group of four values ----
@@ -644,22 +659,25 @@ __global__ void __launch_bounds__(TcShape<D, TILES, QS, KV>::kThreads, 1) tree_t
                 const int l8 = lane & 7;
 #pragma unroll 1
                 for (int r0 = mine * 4 + (lane >> 3); r0 < 128; r0 += NW * 4 * B) {
-                    float q[B][4 * G];
+                    float q[B * G][4];
+                    size_t at[B * G];
 #pragma unroll
                     for (int x = 0; x < B; ++x) {
                         const int pr = seg.rt * RT + tile * 128 + r0 + NW * 4 * x;
                         const bool there = pr < rows;
                         const int i = there ? pr / p.group : 0;
-                        const size_t at = (size_t)(seg.row0 + i) * p.q_stride + (size_t)(seg.kvh * p.group + (there ? pr - i * p.group : 0)) * p.d;
+                        const size_t row = (size_t)(seg.row0 + i) * p.q_stride + (size_t)(seg.kvh * p.group + (there ? pr - i * p.group : 0)) * p.d;
 #pragma unroll
                         for (int g = 0; g < G; ++g) {
-                            float v[4] = {0.f, 0.f, 0.f, 0.f};
                             const int e = 4 * (l8 + 8 * g);
-                            if (there && e < p.d) tree_load<4>(p.q, p.q_type, at + e, v);
-#pragma unroll
-                            for (int k = 0; k < 4; ++k) q[x][4 * g + k] = v[k] * sign;
+                            at[x * G + g] = there && e < p.d ? row + e : kTreeNone;
                         }
                     }
+                    tree_load<4, B * G>(p.q, p.q_type, at, q);
+#pragma unroll
+                    for (int i = 0; i < B * G; ++i)
+#pragma unroll
+                        for (int e = 0; e < 4; ++e) q[i][e] *= sign;
 #pragma unroll
                     for (int x = 0; x < B; ++x) {
                         const int r = r0 + NW * 4 * x;
@@ -667,7 +685,7 @@ __global__ void __launch_bounds__(TcShape<D, TILES, QS, KV>::kThreads, 1) tree_t
                         if (p.q_type != VSPEC_B200_T_F16) {
                             float top = 0.f;
 #pragma unroll
-                            for (int e = 0; e < 4 * G; ++e) top = fmaxf(top, fabsf(q[x][e]));
+                            for (int e = 0; e < 4 * G; ++e) top = fmaxf(top, fabsf(q[x * G + e / 4][e % 4]));
 #pragma unroll
                             for (int o = 4; o > 0; o >>= 1) top = fmaxf(top, __shfl_xor_sync(0xffffffffu, top, o));
                             // 2^ex with the row's largest value in [2^13, 2^14), as far as normal numbers reach
@@ -676,7 +694,7 @@ __global__ void __launch_bounds__(TcShape<D, TILES, QS, KV>::kThreads, 1) tree_t
                             mul = __uint_as_float((uint32_t)(127 + ex) << 23);
                             const float inv = __uint_as_float((uint32_t)(127 - ex) << 23);
 #pragma unroll
-                            for (int e = 0; e < 4 * G; ++e) q[x][e] *= inv;
+                            for (int e = 0; e < 4 * G; ++e) q[x * G + e / 4][e % 4] *= inv;
                         }
                         // a scale of 0: scores of 0 from products of any size, and -inf stays -inf
                         if (l8 == 0) sm.mul[tile * 128 + r] = fmaxf(mul * fabsf(p.scale) * kTreeLog2e, 1e-38f);
@@ -684,7 +702,7 @@ __global__ void __launch_bounds__(TcShape<D, TILES, QS, KV>::kThreads, 1) tree_t
                         for (int g = 0; g < G; ++g) {
                             const int el = 4 * (l8 + 8 * g), ch = el >> 3;
                             unsigned char* at = qt + (ch >> 3) * kTcHalf + r * 128 + (((ch & 7) ^ (r & 7)) << 4) + (el & 4) * 2;
-                            float* v = &q[x][4 * g];
+                            float (&v)[4] = q[x * G + g];
 #pragma unroll
                             for (int s = 0; s < QS; ++s) {
                                 const uint32_t h0 = tree_pack(v[0], v[1]), h1 = tree_pack(v[2], v[3]);
@@ -697,6 +715,16 @@ __global__ void __launch_bounds__(TcShape<D, TILES, QS, KV>::kThreads, 1) tree_t
                 }
                 asm volatile("fence.proxy.async.shared::cta;\n" ::: "memory");
                 mbar_arrive(&sm.q_full);
+                // the next segment, and its q rows into L2, while this one's products begin
+                more = walk.next(p, ahead);
+                if (more) {
+                    const int pr = ahead.rt * RT + (TILES == 2 ? 128 * w : 0) + row;
+                    if ((TILES == 2 || w == 0) && pr < ahead.drafted * p.group) {
+                        const int i = pr / p.group, es = p.q_type == VSPEC_B200_T_F32 ? 4 : 2;
+                        const char* at = (const char*)p.q + ((size_t)(ahead.row0 + i) * p.q_stride + (size_t)(ahead.kvh * p.group + pr - i * p.group) * p.d) * es;
+                        for (int x = 0; x < p.d * es; x += 128) asm volatile("prefetch.global.L2 [%0];\n" ::"l"(at + x));
+                    }
+                }
                 if (!tc_wait(&sm.q_full, q_phase, abort_flag)) { ok = false; break; }
                 q_phase ^= 1u;
             }
@@ -816,11 +844,13 @@ __global__ void __launch_bounds__(TcShape<D, TILES, QS, KV>::kThreads, 1) tree_t
                     } else {
                         tc_st_x8(s_addr + 8u * c, h);
                     }
+                    if (c == 3 || c == 7) {      // half of the step's weights are there
+                        tmem_wait_st();
+                        tc_fence_before();
+                        mbar_arrive(c == 3 ? &sm.p_half[w] : &sm.p_full[w]);
+                    }
                 });
                 l = fmaf(l, f, (ls[0] + ls[1]) + (ls[2] + ls[3]));
-                tmem_wait_st();
-                tc_fence_before();
-                mbar_arrive(&sm.p_full[w]);
             }
             if (!ok) break;
             k_steps += seg.steps;
@@ -865,6 +895,10 @@ __global__ void __launch_bounds__(TcShape<D, TILES, QS, KV>::kThreads, 1) tree_t
                 constexpr int CW = QS * D / 2 < 64 ? QS * D / 2 : 64, LPR = CW / 4;
                 const bool whole = seg.steps == seg.n;
                 const float inv = !whole ? 1.f : (l == 0.f ? 0.f : 1.0f / l);
+                // where this lane's row goes
+                const size_t part = (size_t)(2 * blockIdx.x + (seg.step0 == 0 ? 1 : 0)) * RT + local;
+                const size_t out_at = !in ? kTreeNone : !whole ? part * p.d
+                    : ((size_t)(seg.row0 + ti) * p.hq + (size_t)seg.kvh * p.group + (pr - ti * p.group)) * p.d;
                 float4* stage = reinterpret_cast<float4*>(smem + (TILES == 2 ? w * QS : 0) * S::kSlot + quad * (32 * CW * 4));
 #pragma unroll
                 for (int c = 0; c < D / CW; ++c) {
@@ -877,22 +911,19 @@ __global__ void __launch_bounds__(TcShape<D, TILES, QS, KV>::kThreads, 1) tree_t
                     }
                     __syncwarp();
                     const int piece = lane % LPR, e = CW * c + 4 * piece;
+                    const uint32_t mine_lo = (uint32_t)out_at, mine_hi = (uint32_t)(out_at >> 32);
 #pragma unroll 4
                     for (int i = 0; i < 32; i += 32 / LPR) {
-                        const int r = i + lane / LPR, lr = (TILES == 2 ? 128 * w : 0) + 32 * quad + r, pr2 = seg.rt * RT + lr;
+                        const int r = i + lane / LPR;
                         const float4 v = stage[r * LPR + (piece ^ (r & 7))];
-                        if (pr2 < rows && e < p.d) {
-                            if (whole) {
-                                const int i2 = pr2 / p.group;
-                                tree_store4(p.out, p.q_type, ((size_t)(seg.row0 + i2) * p.hq + (size_t)seg.kvh * p.group + pr2 - i2 * p.group) * p.d + e, v, 1.f, false);
-                            } else {
-                                *reinterpret_cast<float4*>(p.part_o + ((size_t)(2 * blockIdx.x + (seg.step0 == 0 ? 1 : 0)) * RT + lr) * p.d + e) = v;
-                            }
+                        const size_t at = __shfl_sync(0xffffffffu, mine_lo, r) | (size_t)__shfl_sync(0xffffffffu, mine_hi, r) << 32;
+                        if (at != kTreeNone && e < p.d) {
+                            if (whole) tree_store4(p.out, p.q_type, at + e, v, 1.f, false);
+                            else *reinterpret_cast<float4*>(p.part_o + at + e) = v;
                         }
                     }
                 }
-                if (!whole && in)
-                    *reinterpret_cast<float2*>(p.part_ml + ((size_t)(2 * blockIdx.x + (seg.step0 == 0 ? 1 : 0)) * RT + local) * 2) = make_float2(m, l);
+                if (!whole && in) *reinterpret_cast<float2*>(p.part_ml + part * 2) = make_float2(m, l);
             }
             // every warp's stage has been read before any writes the next segment's q there
             uint64_t* read = TILES == 1 ? &sm.pair : &sm.staged[w];
@@ -953,10 +984,10 @@ __global__ void __launch_bounds__(256) tree_tc_combine_kernel(const TreeParams p
     int n, tiles, row0;
     (void)tc_work<RT>(p, b, n, tiles);
     const int drafted = tree_rows(p, b, row0), rows = drafted * p.group;
-    const int pair = (int)((at - before) / n);
-    const long long start = before + (long long)pair * n;
-    if (start == at) return;                   // between two pairs
-    // the CTA of step s: the largest c with total c / g <= s
+    const int units = n + kTcPairCost, pair = (int)((at - before) / units);
+    const long long start = before + (long long)pair * units + kTcPairCost;   // the pair's first step
+    if (at <= start) return;                   // between two pairs
+    // the CTA of unit s: the largest c with total c / g <= s
     const int first = (int)(((start + 1) * g + total - 1) / total) - 1;
     const int last = (int)(((start + n) * g + total - 1) / total) - 1;
     if (first != cut - 1) return;              // not the pair's first cut
