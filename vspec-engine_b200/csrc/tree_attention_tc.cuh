@@ -5,7 +5,7 @@
 // fp16: from a few dozen rows on, warp-level MMA (576 TFLOP/s here) and not DRAM
 // is the bound.  Here one thread issues tcgen05.mma for tiles of 128 rows x 128
 // tokens, with S = Q K^T and O = P V in tensor memory:
-//   warps 0-3, 4-7   softmax, one thread a row (TMEM lane): maximum and
+//   warps 0-3, 4-7   softmax, a row (TMEM lane) a thread: maximum and
 //                    exponentials of S, P back over S as fp16, the step's O
 //                    added to fp32 registers (a step's product starts from 0:
 //                    the tensor cores truncate, see tree_attention_mma.cuh)
@@ -15,8 +15,8 @@
 //                    in a raw ring and are widened to fp16 into the tiles
 // Two tiles are in flight so that the tensor cores work on one while the other
 // is in its softmax: two row tiles sharing each K and V tile when a pair has
-// more than 128 rows (TILES = 2), else alternate steps of one row tile, joined
-// at the end (TILES = 1).
+// more than 128 rows (TILES = 2), else alternate steps of one row tile, with the
+// two softmax groups sharing out a step's tokens and the dims (TILES = 1).
 //
 // The grid is persistent: all pairs' steps, laid out in a row, are cut into
 // equal runs, one a CTA, so that sequences of any lengths balance to one step.
@@ -24,6 +24,8 @@
 // the parts of such pairs in order.  fp32 q and 8-bit pages are split and scaled
 // as in the warp-MMA kernels.
 #pragma once
+
+#include <stddef.h>
 
 #include "tma_map.cuh"
 #include "tree_attention_mma.cuh"
@@ -47,17 +49,19 @@ struct TcParams {
 template <int D, int TILES, int QS, int KV>
 struct TcShape {
     static constexpr int kProducers = KV == kTreeF16 ? 3 : 7;
+    static constexpr int kFillers = KV == kTreeF16 ? 3 : 6;   // warps that hand a tile over
     static constexpr int kThreads = (kTcFirstProducer + kProducers) * 32;
     // registers a thread of the softmax warps (256 threads) and of the others: together what the CTA is launched
     // with, 384 x 168 or 512 x 128
-    static constexpr int kSoftmaxRegs = KV == kTreeF16 ? 216 : 192, kOtherRegs = KV == kTreeF16 ? 72 : 64;
+    static constexpr int kSoftmaxRegs = KV == kTreeF16 ? (TILES == 2 ? 216 : 184) : (TILES == 2 ? 176 : 152);
+    static constexpr int kOtherRegs = KV == kTreeF16 ? (TILES == 2 ? 72 : 136) : (TILES == 2 ? 80 : 104);
     static_assert(256 * kSoftmaxRegs + (kThreads - 256) * kOtherRegs <= kThreads * (65536 / kThreads / 8 * 8), "register split");
     static constexpr uint32_t kSlot = kTcStep * D * 2;
     static constexpr uint32_t kQ = TILES * QS * kSlot;
     static constexpr uint32_t kRaw = KV == kTreeF16 ? 0 : kTcRawSlots * kTcStep * D;
-    static constexpr uint32_t kMisc = KV == kTreeF16 ? 3072 : 7168;
+    static constexpr uint32_t kMisc = KV == kTreeF16 ? (TILES == 2 ? 3072 : 4096) : 8192;
     static constexpr int kFit = (int)((kTcSmemMax - kMisc - kQ - kRaw) / kSlot);
-    static constexpr int kMost = KV == kTreeF16 ? 6 : 4;   // 4: the scale ring below
+    static constexpr int kMost = 6;
     static constexpr int kSlots = kFit < kMost ? kFit : kMost;
     static constexpr uint32_t kRingAt = kQ, kRawAt = kQ + kSlots * kSlot, kMiscAt = kRawAt + kRaw;
     static constexpr uint32_t kTotal = kMiscAt + kMisc;
@@ -67,13 +71,13 @@ struct TcShape {
 // misc area
 struct alignas(16) TcMisc {
     float mul[256];             // score multiplier of each row
-    uint64_t full[6], empty[6], raw_full[kTcRawSlots], raw_empty[kTcRawSlots], s_full[2], p_half[2], p_full[2], q_full, pair, staged[2], drain;
+    uint64_t full[6], empty[6], raw_full[kTcRawSlots], raw_empty[kTcRawSlots], sc_full[4], sc_empty[4], s_full[2], p_half[2], p_full[2], q_full, pair, staged[2], drain;
     uint32_t tmem;
     int abort;
     int start_b;
     long long start_off, total;
     int odd[8];                 // step + 1 where V held infinities or NaN
-    float ml[2][128];           // of the second softmax group (TILES = 1)
+    float row[2][2][128];       // maxima, at last sums, of the two softmax groups (TILES = 1), in turn
 };
 struct alignas(16) TcScales {   // 8-bit pages: scales of four steps, read four at a time
     float k[4][kTcStep], v[4][kTcStep];
@@ -134,13 +138,16 @@ __device__ __forceinline__ void tc_landed(float (&v)[16]) {
                    "+f"(v[8]), "+f"(v[9]), "+f"(v[10]), "+f"(v[11]), "+f"(v[12]), "+f"(v[13]), "+f"(v[14]), "+f"(v[15])
                  :: "memory");
 }
-// f(c, v) for N chunks of 16 TMEM columns of this thread's lane, the next chunk's load in flight.
-template <int N, typename F>
+// f(c, v) for N chunks of 16 TMEM columns of this thread's lane, the next
+// chunk's load in flight.  UNROLL: c is a constant in f (it indexes registers);
+// else a loop of two chunks, which keeps the code of a step in the instruction
+// cache.
+template <int N, bool UNROLL, typename F>
 __device__ __forceinline__ void tc_sweep(uint32_t taddr, F f) {
     static_assert(N % 2 == 0, "pairs of chunks");
     float a[16], b[16];
     tmem_ld_x16(taddr, a);
-#pragma unroll
+#pragma unroll (UNROLL ? N / 2 : 1)
     for (int c = 0; c < N; c += 2) {
         tc_landed(a);
         tmem_ld_x16(taddr + 16u * (c + 1), b);
@@ -260,17 +267,15 @@ __global__ void __launch_bounds__(TcShape<D, TILES, QS, KV>::kThreads, 1) tree_t
     TcMisc& sm = *reinterpret_cast<TcMisc*>(smem + S::kMiscAt);
     TcScales& sc = *reinterpret_cast<TcScales*>(smem + S::kMiscAt + sizeof(TcMisc));
     static_assert(sizeof(TcMisc) % 16 == 0 && S::kMiscAt % 16 == 0, "vector reads of the scales behind");
-    static_assert(sizeof(TcMisc) + (KV == kTreeF16 ? 0 : sizeof(TcScales)) <= S::kMisc, "misc area");
+    static_assert((TILES == 2 ? offsetof(TcMisc, row) : sizeof(TcMisc)) + (KV == kTreeF16 ? 0 : sizeof(TcScales)) <= S::kMisc, "misc area");
     const int tid = threadIdx.x, warp = tid >> 5, lane = tid & 31;
     volatile int* abort_flag = &sm.abort;
-    pdl_wait();
-    pdl_trigger();
 
-    // ---- this CTA's run ----
     if (tid == 0) {
         sm.abort = 0;
-        for (int i = 0; i < 6; ++i) { mbar_init(&sm.full[i], kTcProducers); mbar_init(&sm.empty[i], 1); }
-        for (int i = 0; i < kTcRawSlots; ++i) { mbar_init(&sm.raw_full[i], 1); mbar_init(&sm.raw_empty[i], kTcProducers); }
+        for (int i = 0; i < 6; ++i) { mbar_init(&sm.full[i], S::kFillers); mbar_init(&sm.empty[i], 1); }
+        for (int i = 0; i < kTcRawSlots; ++i) { mbar_init(&sm.raw_full[i], 1); mbar_init(&sm.raw_empty[i], S::kFillers); }
+        for (int i = 0; i < 4; ++i) { mbar_init(&sm.sc_full[i], 1); mbar_init(&sm.sc_empty[i], 8); }
         for (int i = 0; i < 2; ++i) { mbar_init(&sm.s_full[i], 1); mbar_init(&sm.p_half[i], 128); mbar_init(&sm.p_full[i], 128); }
         mbar_init(&sm.q_full, 256);
         mbar_init(&sm.pair, 256);
@@ -282,6 +287,10 @@ __global__ void __launch_bounds__(TcShape<D, TILES, QS, KV>::kThreads, 1) tree_t
         tma_prefetch_desc(&pp.v_map);
     }
     if (KV != kTreeF16 && tid < kTcStep) sc.one[tid] = 1.0f;
+    pdl_wait();
+    pdl_trigger();
+
+    // ---- this CTA's run ----
     long long lo = 0, hi = 0;
     if (warp == 0) {
         long long total = 0;
@@ -345,7 +354,6 @@ __global__ void __launch_bounds__(TcShape<D, TILES, QS, KV>::kThreads, 1) tree_t
         const int br = pp.box_rows, boxes = kTcStep / br;      // boxes of a whole tile: 1 to 16
         int slot = 0, raw = 0;
         uint32_t phase = 0, raw_phase = 0;   // of the slot's next use
-        uint32_t raw_used = 0;               // raw slots used before, and from bit 8 the phases of their release
         bool wrapped = false;                // the ring has been filled once
         int k_steps = 0;                     // steps of the CTA's run before this segment
         auto advance = [&]() {
@@ -362,12 +370,12 @@ __global__ void __launch_bounds__(TcShape<D, TILES, QS, KV>::kThreads, 1) tree_t
             const int32_t* table = p.table + (size_t)seg.b * p.max_pages;
             const int total = seg.ctx + seg.drafted, t_first = seg.step0 * kTcStep;
             const int loads = TILES == 2 ? 2 * seg.steps : 2 * seg.steps + 1;
-            // pool row of box `lane` of step j, a step ahead of its use
+            // page of box `lane` of step j, loaded two steps ahead of its use and looked at only then
             auto find = [&](int j) -> int {
-                const int t = t_first + j * kTcStep + lane * br;
-                return j < seg.steps && lane < boxes && t < total ? tree_pool_row(p, table, t) : 0;
+                const int t = min(t_first + j * kTcStep + lane * br, total - 1);
+                return __ldg(table + min(t / p.page_tokens, p.max_pages - 1));
             };
-            int row_even = find(0), row_odd = find(1);
+            int page_even = find(0), page_odd = find(1);
             // the boxes of K or V of step j
             auto issue = [&](bool is_v, int j, uint32_t dst, uint64_t* bar) {
                 const int left = total - (t_first + j * kTcStep);
@@ -375,7 +383,13 @@ __global__ void __launch_bounds__(TcShape<D, TILES, QS, KV>::kThreads, 1) tree_t
                 constexpr uint32_t kRowBytes = KV == kTreeF16 ? D * 2 : D;
                 if (lane == 0) mbar_arrive_expect_tx(bar, (uint32_t)(nb * br) * kRowBytes);
                 __syncwarp();
-                const int row = (j & 1) ? row_odd : row_even;
+                const int t = min(t_first + j * kTcStep + lane * br, total - 1), at = t / p.page_tokens;
+                int page = (j & 1) ? page_odd : page_even;
+                if (at >= p.max_pages || page < 0 || page >= p.num_pages) {
+                    if (lane < nb) atomicOr(p.fault, 1);
+                    page = 0;
+                }
+                const int row = page * p.page_tokens + (t - at * p.page_tokens);
                 const CUtensorMap* map = is_v ? &pp.v_map : &pp.k_map;
                 if (lane < nb) {
                     if (KV == kTreeF16) {
@@ -386,10 +400,9 @@ __global__ void __launch_bounds__(TcShape<D, TILES, QS, KV>::kThreads, 1) tree_t
                         tc_tma_3d(dst + (uint32_t)(lane * br) * D, map, 0, seg.kvh, row, bar);
                     }
                 }
-                // K and V of a step share its rows: after V they are those of the step after next
+                // K and V of a step share its pages: after V they are those of the step after next
                 if (is_v) {
-                    const int next = find(j + 2);
-                    if (j & 1) row_odd = next; else row_even = next;
+                    if (j & 1) page_odd = find(j + 2); else page_even = find(j + 2);
                 }
             };
             const uint32_t ring = smem_u32(smem) + S::kRingAt;
@@ -434,31 +447,67 @@ __global__ void __launch_bounds__(TcShape<D, TILES, QS, KV>::kThreads, 1) tree_t
                     advance();
                 }
             } else {
-                // codes of load li land in raw slot `raw`, three loads ahead of the conversion
-                auto issue_raw = [&](int li, int to) {
-                    bool is_v;
-                    int j;
-                    decode(li, is_v, j);
-                    if (pw == 0 && li < loads && j < seg.steps) {
-                        // every warp has read what the slot held
-                        if ((raw_used >> to) & 1u) {
-                            if (!tc_wait(&sm.raw_empty[to], (raw_used >> (8 + to)) & 1u, abort_flag)) ok = false;
-                            raw_used ^= 256u << to;
+                // The first warp has codes land in the raw ring, as far ahead as it reaches, and fetches the scales; the
+                // others widen the codes.  (With page lookups and scales on a widening warp, that warp was the step's
+                // longest path: 6300 cycles.)
+                if (pw == 0) {
+                    // Scales of K and V of a step's tokens, four a lane, in registers a step ahead and then in a ring of
+                    // their own.  Every load is issued whatever its token, so that all are in flight at once.
+                    float ks[4], vs[4];
+                    int spage[4];                            // pages of the step after
+                    auto token = [&](int j, int q) { return t_first + j * kTcStep + 32 * q + lane; };
+                    auto fetch_pages = [&](int j) {
+#pragma unroll
+                        for (int q = 0; q < 4; ++q)
+                            spage[q] = __ldg(table + min(min(token(j, q), total - 1) / p.page_tokens, p.max_pages - 1));
+                    };
+                    auto fetch_scales = [&](int j) {         // from spage
+#pragma unroll
+                        for (int q = 0; q < 4; ++q) {
+                            const int t = min(token(j, q), total - 1), at = t / p.page_tokens;
+                            const bool bad = at >= p.max_pages || spage[q] < 0 || spage[q] >= p.num_pages;   // noted with the boxes
+                            const size_t r = (size_t)((bad ? 0 : spage[q]) * p.page_tokens + (t - at * p.page_tokens)) * p.hkv + seg.kvh;
+                            ks[q] = __ldg(p.k_scales + r);
+                            vs[q] = __ldg(p.v_scales + r);
                         }
-                        raw_used |= 1u << to;
-                        if (ok) issue(is_v, j, smem_u32(smem) + S::kRawAt + (uint32_t)to * (kTcStep * D), &sm.raw_full[to]);
+                    };
+                    fetch_pages(0);
+                    fetch_scales(0);
+                    fetch_pages(1);
+                    for (int li = 0; li < loads && ok; ++li) {
+                        bool is_v;
+                        int j;
+                        decode(li, is_v, j);
+                        if (j >= seg.steps) continue;
+                        if (wrapped && !tc_wait(&sm.raw_empty[raw], raw_phase ^ 1u, abort_flag)) { ok = false; break; }
+                        issue(is_v, j, smem_u32(smem) + S::kRawAt + (uint32_t)raw * (kTcStep * D), &sm.raw_full[raw]);
+                        if (++raw == kTcRawSlots) { raw = 0; raw_phase ^= 1u; wrapped = true; }
+                        if (is_v) continue;
+                        const int k = k_steps + j, e = k & 3;
+                        if (k >= 4 && !tc_wait(&sm.sc_empty[e], (uint32_t)((k >> 2) - 1) & 1u, abort_flag)) { ok = false; break; }
+                        const bool drafted = t_first + (j + 1) * kTcStep > seg.ctx;
+                        float top = 0.f;
+#pragma unroll
+                        for (int q = 0; q < 4; ++q) {
+                            if (token(j, q) >= total) ks[q] = vs[q] = 0.f;
+                            // a V scale that is not finite reaches the rows that see its token as its values do
+                            if (!(vs[q] <= 3.402823466e+38f) && drafted) { sm.odd[k & 7] = k + 1; vs[q] = 0.f; }
+                            sc.k[e][32 * q + lane] = ks[q];
+                            sc.v[e][32 * q + lane] = vs[q];
+                            if (vs[q] <= 3.402823466e+38f) top = fmaxf(top, vs[q]);
+                        }
+                        top = warp_max(top);
+                        int ex = -100;
+                        if (top > 0.f) (void)frexpf(top, &ex);
+                        if (lane == 0) sc.v_exp[e] = max(ex, -100);
+                        __syncwarp();
+                        if (lane == 0) mbar_arrive(&sm.sc_full[e]);
+                        fetch_scales(j + 1);
+                        fetch_pages(j + 2);
                     }
-                    return li < loads && j < seg.steps;
-                };
-                // loads that exist, in order: the raw ring counts those alone
-                int ahead = 0, to = raw;
-                auto step_ahead = [&]() {
-                    while (ahead < loads && !issue_raw(ahead, to)) ++ahead;
-                    if (ahead < loads) { ++ahead; to = to + 1 == kTcRawSlots ? 0 : to + 1; }
-                };
-                step_ahead();
-                step_ahead();
-                step_ahead();
+                    k_steps += seg.steps;
+                    continue;
+                }
                 for (int li = 0; li < loads && ok; ++li) {
                     bool is_v;
                     int j;
@@ -466,27 +515,24 @@ __global__ void __launch_bounds__(TcShape<D, TILES, QS, KV>::kThreads, 1) tree_t
                     if (j >= seg.steps) continue;
                     const int t0 = t_first + j * kTcStep;
                     const bool drafted = t0 + kTcStep > seg.ctx;
-                    // scales of step j: the K load carries those of K and V
-                    float ks[4], vs[4];
-                    const bool scales = !is_v && pw == kTcProducers - 1;
-                    if (scales) {
-#pragma unroll
-                        for (int q = 0; q < 4; ++q) {
-                            const int t = t0 + 32 * q + lane;
-                            const int r = t < total ? tree_pool_row(p, table, t) : -1;
-                            ks[q] = r < 0 ? 0.f : __ldg(p.k_scales + (size_t)r * p.hkv + seg.kvh);
-                            vs[q] = r < 0 ? 0.f : __ldg(p.v_scales + (size_t)r * p.hkv + seg.kvh);
-                        }
-                    }
-                    if (!tc_wait(&sm.raw_full[raw], (raw_phase >> raw) & 1u, abort_flag) || !wait_slot()) { ok = false; break; }
+                    if (!tc_wait(&sm.raw_full[raw], raw_phase, abort_flag) || !wait_slot()) { ok = false; break; }
                     unsigned char* st = smem + S::kRingAt + (uint32_t)slot * S::kSlot;
                     const unsigned char* rs = smem + S::kRawAt + raw * (kTcStep * D);
                     const int there = min(total - t0, kTcStep);
                     bool odd = false;
-#pragma unroll 2
-                    for (int i = pw * 32 + lane; i < kTcStep * (D / 16); i += kTcProducers * 32) {
+                    constexpr int PIECES = kTcStep * (D / 16), LANES = S::kFillers * 32, MINE = (PIECES + LANES - 1) / LANES;
+                    uint4 code[MINE];
+#pragma unroll
+                    for (int x = 0; x < MINE; ++x) {
+                        const int i = min((pw - 1) * 32 + lane + x * LANES, PIECES - 1);
+                        code[x] = *reinterpret_cast<const uint4*>(rs + i * 16);
+                    }
+#pragma unroll
+                    for (int x = 0; x < MINE; ++x) {
+                        const int i = (pw - 1) * 32 + lane + x * LANES;
+                        if (i >= PIECES) break;
                         const int r = i / (D / 16), pc = i % (D / 16);
-                        uint4 c = *reinterpret_cast<const uint4*>(rs + i * 16);
+                        uint4 c = code[x];
                         if (drafted && r >= there) c = make_uint4(0, 0, 0, 0);
                         uint4 a, b;
                         tree_widen<KV>(c.x, a.x, a.y);
@@ -498,35 +544,19 @@ __global__ void __launch_bounds__(TcShape<D, TILES, QS, KV>::kThreads, 1) tree_t
                             tc_clear_odd(a);
                             tc_clear_odd(b);
                         }
-                        unsigned char* row = st + (pc >> 2) * kTcHalf + r * 128;
-                        const int ch = (2 * pc) & 7;
-                        *reinterpret_cast<uint4*>(row + ((ch ^ (r & 7)) << 4)) = a;
-                        *reinterpret_cast<uint4*>(row + (((ch + 1) ^ (r & 7)) << 4)) = b;
-                    }
-                    if (scales) {
-                        const int e = (k_steps + j) & 3;
-                        float top = 0.f;
-#pragma unroll
-                        for (int q = 0; q < 4; ++q) {
-                            // a V scale that is not finite reaches the rows that see its token as its values do
-                            if (!(vs[q] <= 3.402823466e+38f) && drafted) { odd = true; vs[q] = 0.f; }
-                            sc.k[e][32 * q + lane] = ks[q];
-                            sc.v[e][32 * q + lane] = vs[q];
-                            if (vs[q] <= 3.402823466e+38f) top = fmaxf(top, vs[q]);
-                        }
-                        top = warp_max(top);
-                        int ex = -100;
-                        if (top > 0.f) (void)frexpf(top, &ex);
-                        if (lane == 0) sc.v_exp[e] = max(ex, -100);
+                        // the two halves of 64 dims lie in the same banks: lanes of the second store their chunks in the
+                        // other order, so that eight lanes cover all banks
+                        const int h = pc >> 2, ch = (2 * pc) & 7;
+                        unsigned char* row = st + h * kTcHalf + r * 128;
+                        *reinterpret_cast<uint4*>(row + (((ch + h) ^ (r & 7)) << 4)) = h ? b : a;
+                        *reinterpret_cast<uint4*>(row + (((ch + 1 - h) ^ (r & 7)) << 4)) = h ? a : b;
                     }
                     if (odd) sm.odd[(k_steps + j) & 7] = k_steps + j + 1;
                     asm volatile("fence.proxy.async.shared::cta;\n" ::: "memory");
                     __syncwarp();
                     if (lane == 0) { mbar_arrive(&sm.full[slot]); mbar_arrive(&sm.raw_empty[raw]); }
                     advance();
-                    raw_phase ^= 1u << raw;
-                    raw = raw + 1 == kTcRawSlots ? 0 : raw + 1;
-                    step_ahead();
+                    if (++raw == kTcRawSlots) { raw = 0; raw_phase ^= 1u; }
                 }
             }
             k_steps += seg.steps;
@@ -571,7 +601,7 @@ __global__ void __launch_bounds__(TcShape<D, TILES, QS, KV>::kThreads, 1) tree_t
                     for (int k1 = 0; k1 < 2; ++k1)
 #pragma unroll
                         for (int q = 0; q < QS; ++q)
-                            tc_mma_ts(d, a + 8u * (QS * (2 * k2 + k1) + q), vb + (uint32_t)(2 * k2 + k1) * TOKENS, idesc_o, k2 || k1 || q);
+                            tc_mma_ts(d, a + 64u * half + 8u * (QS * (2 * (k2 & 1) + k1) + q), vb + (uint32_t)(2 * k2 + k1) * TOKENS, idesc_o, k2 || k1 || q);
             };
             // the two halves of a step's weights have a barrier each: one barrier's second completion would hide the first
             auto wait_p = [&](int w, int half) -> bool {
@@ -641,7 +671,6 @@ __global__ void __launch_bounds__(TcShape<D, TILES, QS, KV>::kThreads, 1) tree_t
         tc_regs_inc<S::kSoftmaxRegs>();
         const int w = warp >> 2, quad = warp & 3, row = 32 * quad + lane;
         const uint32_t lanes = (uint32_t)(32 * quad) << 16;
-        const uint32_t s_addr = tmem + lanes + 128u * w, o_addr = tmem + lanes + 256u + 128u * w;
         uint32_t q_phase = 0, s_phase = 0, pair_phase = 0, staged_phase = 0;
         int k_steps = 0;
         TcSegment ahead;
@@ -733,29 +762,34 @@ __global__ void __launch_bounds__(TcShape<D, TILES, QS, KV>::kThreads, 1) tree_t
             const bool in = pr < rows;
             const int ti = in ? pr / p.group : 0;
             const float mul = sm.mul[local];
-            float o[D];
+            // TILES = 2: this thread has its row's 128 tokens of a step and all dims.  TILES = 1: 64 of the tokens and half
+            // of the dims, the other group the rest; the two agree on a step's maximum, and steps alternate between the two
+            // S and O buffers, whose products are a step ahead.
+            constexpr int OD = TILES == 2 ? D : D / 2, NC = TILES == 2 ? 8 : 4, LAG = TILES == 2 ? 1 : 2;
+            const int col0 = TILES == 2 ? 0 : 64 * w, dim0 = TILES == 2 ? 0 : OD * w;
+            float o[OD];
 #pragma unroll
-            for (int i = 0; i < D; ++i) o[i] = 0.f;
-            float m = kTreeLowest, l = 0.f, f = 1.f;
-            int v_exp = -100, prev_j = -1;
-            // the product of the step before: o = o f + P V
-            auto add_o = [&]() {
-                const int tag = k_steps + prev_j + 1;
-                tc_sweep<D / 16>(o_addr, [&](int c, float (&v)[16]) {
+            for (int i = 0; i < OD; ++i) o[i] = 0.f;
+            float m = kTreeLowest, l = 0.f, f_even = 1.f, f_odd = 1.f;
+            int v_exp = -100;
+            // the product of step j: o = o f + P V
+            auto add_o = [&](int j, int u, float f) {
+                const int tag = k_steps + j + 1;
+                tc_sweep<OD / 16, true>(tmem + lanes + 256u + 128u * u + (uint32_t)dim0, [&](int c, float (&v)[16]) {
 #pragma unroll
                     for (int i = 0; i < 16; ++i) o[16 * c + i] = fmaf(o[16 * c + i], f, v[i]);
                 });
                 if (sm.odd[(tag - 1) & 7] == tag) {
                     // infinities and NaN among the step's drafted tokens, for the rows that see them
                     const int32_t* table = p.table + (size_t)seg.b * p.max_pages;
-                    const int t0 = (seg.step0 + prev_j) * kTcStep;
+                    const int t0 = (seg.step0 + j) * kTcStep;
                     for (int t = max(t0, seg.ctx); t < min(t0 + kTcStep, seg.ctx + seg.drafted); ++t) {
                         if (!in || !tree_sees(p, seg.row0, ti, seg.ctx, seg.drafted, t)) continue;
-                        const size_t head = (size_t)tree_pool_row(p, table, t) * p.hkv + seg.kvh, at = head * p.d;
+                        const size_t head = (size_t)tree_pool_row(p, table, t) * p.hkv + seg.kvh, at = head * p.d + dim0;
                         const float vs = KV == kTreeF16 ? 1.f : __ldg(p.v_scales + head);
 #pragma unroll
-                        for (int i = 0; i < D; ++i) {
-                            if (i >= p.d) continue;
+                        for (int i = 0; i < OD; ++i) {
+                            if (dim0 + i >= p.d) continue;
                             float v;
                             if (KV == kTreeF16) {
                                 v = __half2float(reinterpret_cast<const __half*>(p.v_pages)[at + i]);
@@ -769,23 +803,27 @@ __global__ void __launch_bounds__(TcShape<D, TILES, QS, KV>::kThreads, 1) tree_t
                     }
                 }
             };
-            const int n = TILES == 2 ? seg.steps : (seg.steps - w + 1) / 2;
-            // one pass more than steps: it adds the last step's product
-            for (int i = 0; i <= n && n > 0; ++i) {
-                const int j = TILES == 2 ? i : 2 * i + w;
-                if (!tc_wait(&sm.s_full[w], s_phase, abort_flag)) { ok = false; break; }
-                s_phase ^= 1u;
-                tc_fence_after();
-                if (i > 0) add_o();
-                if (i == n) break;
-                prev_j = j;
-                const int t0 = (seg.step0 + j) * kTcStep, e4 = (k_steps + j) & 3;
-                const bool masked = t0 + kTcStep > seg.ctx;
-                const float* ks = KV == kTreeF16 ? nullptr : sc.k[e4];
+            const int n = seg.steps;
+            // LAG passes more than steps: they add the last products
+            for (int i = 0; i < n + LAG; ++i) {
+                const int u = TILES == 2 ? w : i & 1;
+                if (i < n || i >= LAG) {
+                    if (!tc_wait(&sm.s_full[u], (s_phase >> u) & 1u, abort_flag)) { ok = false; break; }
+                    s_phase ^= 1u << u;
+                    tc_fence_after();
+                }
+                const bool even = TILES == 2 || u == 0;
+                if (i >= LAG) add_o(i - LAG, u, even ? f_even : f_odd);
+                if (i >= n) continue;
+                const uint32_t s_addr = tmem + lanes + 128u * u + (uint32_t)col0;
+                const int t0 = (seg.step0 + i) * kTcStep + col0, e4 = (k_steps + i) & 3;
+                const bool masked = (seg.step0 + i + 1) * kTcStep > seg.ctx;
+                if (KV != kTreeF16 && !tc_wait(&sm.sc_full[e4], (uint32_t)((k_steps + i) >> 2) & 1u, abort_flag)) { ok = false; break; }
+                const float* ks = KV == kTreeF16 ? nullptr : sc.k[e4] + col0;
                 if (masked) {
                     // what the row does not see becomes -inf in S; the scales of K are applied on the way
 #pragma unroll 1
-                    for (int c = 0; c < 8; ++c) {
+                    for (int c = 0; c < NC; ++c) {
                         float v[16];
                         tmem_ld_x16(s_addr + 16u * c, v);
                         const uint32_t see = in ? tc_sees32(p, seg.row0, ti, seg.drafted, t0 + 16 * c - seg.ctx) : 0u;
@@ -803,14 +841,24 @@ __global__ void __launch_bounds__(TcShape<D, TILES, QS, KV>::kThreads, 1) tree_t
                 }
                 // ---- maximum ----
                 float tops[2] = {-INFINITY, -INFINITY};
-                tc_sweep<8>(s_addr, [&](int c, float (&v)[16]) {
+                tc_sweep<NC, false>(s_addr, [&](int c, float (&v)[16]) {
                     tc_scale<KV != kTreeF16>(v, ks + 16 * c);
 #pragma unroll
                     for (int x = 0; x < 16; ++x) tops[x & 1] = fmaxf(tops[x & 1], v[x]);
                 });
-                const float top = fmaxf(tops[0], tops[1]);
+                float top = fmaxf(tops[0], tops[1]);
+                if (TILES == 1) {
+                    // behind this wait the other group has read its part of the O buffer, too
+                    sm.row[i & 1][w][row] = top;
+                    tc_fence_before();
+                    mbar_arrive(&sm.pair);
+                    if (!tc_wait(&sm.pair, pair_phase, abort_flag)) { ok = false; break; }
+                    pair_phase ^= 1u;
+                    tc_fence_after();
+                    top = fmaxf(top, sm.row[i & 1][w ^ 1][row]);
+                }
                 const float m_new = top == -INFINITY ? m : fmaxf(m, top * mul);
-                f = tree_ex2(m - m_new);
+                float f = tree_ex2(m - m_new);
                 m = m_new;
                 if (KV != kTreeF16) {
                     const int ex = sc.v_exp[e4];
@@ -819,112 +867,94 @@ __global__ void __launch_bounds__(TcShape<D, TILES, QS, KV>::kThreads, 1) tree_t
                         v_exp = ex;
                     }
                 }
+                if (even) f_even = f; else f_odd = f;
                 // ---- weights 2^(s - m + 14 - v_exp), over S: 16 tokens at a time ----
                 const float bias = (KV == kTreeF16 ? 14.f : (float)(14 - v_exp)) - m_new;
                 float ls[4] = {0.f, 0.f, 0.f, 0.f};
-                tc_sweep<8>(s_addr, [&](int c, float (&v)[16]) {
+                tc_sweep<NC, false>(s_addr, [&](int c, float (&v)[16]) {
                     tc_scale<KV != kTreeF16>(v, ks + 16 * c);
 #pragma unroll
                     for (int x = 0; x < 16; ++x) v[x] = tree_ex2(fmaf(v[x], mul, bias));
 #pragma unroll
                     for (int x = 0; x < 16; ++x) ls[x & 3] += v[x];
-                    tc_scale<KV != kTreeF16>(v, &sc.v[e4][16 * c]);
+                    tc_scale<KV != kTreeF16>(v, &sc.v[e4][col0 + 16 * c]);
                     uint32_t h[8];
 #pragma unroll
                     for (int x = 0; x < 8; ++x) h[x] = tree_pack(v[2 * x], v[2 * x + 1]);
+                    // 8 columns of high parts, then 8 of low parts; each half of the tokens in its own half of S
+                    const uint32_t to = s_addr + (uint32_t)((c >> 2) * 64 + (c & 3) * 8 * QS);
+                    tc_st_x8(to, h);
                     if constexpr (QS == 2) {
-                        // 8 columns of high parts, 8 of low parts
-                        tc_st_x8(s_addr + 16u * c, h);
 #pragma unroll
                         for (int x = 0; x < 8; ++x) {
-                            const float2 u = tree_unpack(h[x]);
-                            h[x] = tree_pack(v[2 * x] - u.x, v[2 * x + 1] - u.y);
+                            const float2 y = tree_unpack(h[x]);
+                            h[x] = tree_pack(v[2 * x] - y.x, v[2 * x + 1] - y.y);
                         }
-                        tc_st_x8(s_addr + 16u * c + 8u, h);
-                    } else {
-                        tc_st_x8(s_addr + 8u * c, h);
+                        tc_st_x8(to + 8u, h);
                     }
-                    if (c == 3 || c == 7) {      // half of the step's weights are there
+                    if ((c & 3) == 3) {      // half of the step's weights are there
                         tmem_wait_st();
                         tc_fence_before();
-                        mbar_arrive(c == 3 ? &sm.p_half[w] : &sm.p_full[w]);
+                        mbar_arrive((TILES == 2 ? c == 3 : w == 0) ? &sm.p_half[u] : &sm.p_full[u]);
                     }
                 });
                 l = fmaf(l, f, (ls[0] + ls[1]) + (ls[2] + ls[3]));
+                if (KV != kTreeF16) {
+                    __syncwarp();
+                    if (lane == 0) mbar_arrive(&sm.sc_empty[e4]);
+                }
             }
             if (!ok) break;
-            k_steps += seg.steps;
-            // ---- the rows: natural scale, the two groups' halves joined, out ----
+            k_steps += n;
+            // ---- the rows: natural scale, out ----
             const float unit = ldexpf(1.0f / kTreePScale, KV == kTreeF16 ? 0 : v_exp);
             l *= unit;
 #pragma unroll
-            for (int i = 0; i < D; ++i) o[i] *= unit;
+            for (int i = 0; i < OD; ++i) o[i] *= unit;
             if (TILES == 1) {
-                if (w == 1) {
-                    sm.ml[0][row] = m;
-                    sm.ml[1][row] = l;
-#pragma unroll
-                    for (int c = 0; c < D / 32; ++c) {
-                        uint32_t h[32];
-#pragma unroll
-                        for (int i = 0; i < 32; ++i) h[i] = __float_as_uint(o[32 * c + i]);
-                        tmem_st_x32(o_addr + 32u * c, h);
-                    }
-                    tmem_wait_st();
-                }
-                tc_fence_before();
+                // the weights of the other group's tokens
+                sm.row[n & 1][w][row] = l;
                 mbar_arrive(&sm.pair);
                 if (!tc_wait(&sm.pair, pair_phase, abort_flag)) { ok = false; break; }
                 pair_phase ^= 1u;
-                tc_fence_after();
-                if (w == 0) {
-                    const float m1 = sm.ml[0][row], l1 = sm.ml[1][row];
-                    const float M = fmaxf(m, m1), f0 = tree_ex2(m - M), f1 = tree_ex2(m1 - M);
-                    m = M;
-                    l = l * f0 + l1 * f1;
-                    tc_sweep<D / 16>(o_addr + 128u, [&](int c, float (&v)[16]) {
-#pragma unroll
-                        for (int i = 0; i < 16; ++i) o[16 * c + i] = o[16 * c + i] * f0 + v[i] * f1;
-                    });
-                }
-                tc_fence_before();           // the wait below: the second group's O and (m, l) have been read
+                l += sm.row[n & 1][w ^ 1][row];
             }
-            if (TILES == 2 || w == 0) {
-                // rows out through this warp's quarter of the q tile, whose products are done, CW values of each at a
-                // time: a lane puts its row in, then lanes side by side store pieces of one row
-                constexpr int CW = QS * D / 2 < 64 ? QS * D / 2 : 64, LPR = CW / 4;
-                const bool whole = seg.steps == seg.n;
-                const float inv = !whole ? 1.f : (l == 0.f ? 0.f : 1.0f / l);
-                // where this lane's row goes
-                const size_t part = (size_t)(2 * blockIdx.x + (seg.step0 == 0 ? 1 : 0)) * RT + local;
-                const size_t out_at = !in ? kTreeNone : !whole ? part * p.d
-                    : ((size_t)(seg.row0 + ti) * p.hq + (size_t)seg.kvh * p.group + (pr - ti * p.group)) * p.d;
-                float4* stage = reinterpret_cast<float4*>(smem + (TILES == 2 ? w * QS : 0) * S::kSlot + quad * (32 * CW * 4));
+            // rows out through this warp's part of the q tile, whose products are done, CW values of each at a time: a
+            // lane puts its row in, then lanes side by side store pieces of one row
+            constexpr int kStageWarps = TILES == 2 ? 4 : 8;
+            constexpr int CW = QS * S::kSlot / (kStageWarps * 128) < 64 ? QS * S::kSlot / (kStageWarps * 128) : 64, LPR = CW / 4;
+            const bool whole = seg.steps == seg.n;
+            const size_t part = (size_t)(2 * blockIdx.x + (seg.step0 == 0 ? 1 : 0)) * RT + local;
+            const float inv = !whole ? 1.f : (l == 0.f ? 0.f : 1.0f / l);
+            // where this lane's row goes
+            const size_t out_at = !in ? kTreeNone : !whole ? part * p.d
+                : ((size_t)(seg.row0 + ti) * p.hq + (size_t)seg.kvh * p.group + (pr - ti * p.group)) * p.d;
+            const uint32_t mine_lo = (uint32_t)out_at, mine_hi = (uint32_t)(out_at >> 32);
+            float4* stage = reinterpret_cast<float4*>(smem + (TILES == 2 ? w * QS : 0) * S::kSlot + (TILES == 2 ? quad : warp) * (32 * CW * 4));
+            constexpr int SW = LPR < 8 ? LPR - 1 : 7;
 #pragma unroll
-                for (int c = 0; c < D / CW; ++c) {
-                    __syncwarp();
+            for (int c = 0; c < OD / CW; ++c) {
+                __syncwarp();
 #pragma unroll
-                    for (int i = 0; i < LPR; ++i) {
-                        const float* v = o + CW * c + 4 * i;
-                        stage[lane * LPR + (i ^ (lane & 7))] = whole && l == 0.f ? make_float4(0.f, 0.f, 0.f, 0.f)
-                            : make_float4(v[0] * inv, v[1] * inv, v[2] * inv, v[3] * inv);
-                    }
-                    __syncwarp();
-                    const int piece = lane % LPR, e = CW * c + 4 * piece;
-                    const uint32_t mine_lo = (uint32_t)out_at, mine_hi = (uint32_t)(out_at >> 32);
+                for (int i = 0; i < LPR; ++i) {
+                    const float* v = o + CW * c + 4 * i;
+                    stage[lane * LPR + (i ^ (lane & SW))] = whole && l == 0.f ? make_float4(0.f, 0.f, 0.f, 0.f)
+                        : make_float4(v[0] * inv, v[1] * inv, v[2] * inv, v[3] * inv);
+                }
+                __syncwarp();
+                const int piece = lane % LPR, e = dim0 + CW * c + 4 * piece;
 #pragma unroll 4
-                    for (int i = 0; i < 32; i += 32 / LPR) {
-                        const int r = i + lane / LPR;
-                        const float4 v = stage[r * LPR + (piece ^ (r & 7))];
-                        const size_t at = __shfl_sync(0xffffffffu, mine_lo, r) | (size_t)__shfl_sync(0xffffffffu, mine_hi, r) << 32;
-                        if (at != kTreeNone && e < p.d) {
-                            if (whole) tree_store4(p.out, p.q_type, at + e, v, 1.f, false);
-                            else *reinterpret_cast<float4*>(p.part_o + at + e) = v;
-                        }
+                for (int i = 0; i < 32; i += 32 / LPR) {
+                    const int r = i + lane / LPR;
+                    const float4 v = stage[r * LPR + (piece ^ (r & SW))];
+                    const size_t at = __shfl_sync(0xffffffffu, mine_lo, r) | (size_t)__shfl_sync(0xffffffffu, mine_hi, r) << 32;
+                    if (at != kTreeNone && e < p.d) {
+                        if (whole) tree_store4(p.out, p.q_type, at + e, v, 1.f, false);
+                        else *reinterpret_cast<float4*>(p.part_o + at + e) = v;
                     }
                 }
-                if (!whole && in) *reinterpret_cast<float2*>(p.part_ml + part * 2) = make_float2(m, l);
             }
+            if (!whole && in && (TILES == 2 || w == 0)) *reinterpret_cast<float2*>(p.part_ml + part * 2) = make_float2(m, l);
             // every warp's stage has been read before any writes the next segment's q there
             uint64_t* read = TILES == 1 ? &sm.pair : &sm.staged[w];
             mbar_arrive(read);
@@ -943,11 +973,12 @@ __global__ void __launch_bounds__(TcShape<D, TILES, QS, KV>::kThreads, 1) tree_t
 // Joins the parts of the pairs that were cut.  Block column x stands for the cut
 // between CTAs x and x + 1; the first cut within a pair joins all its parts, in
 // order: the first is in the second part slot of its CTA, the others in the
-// first of theirs.  Eight warps of a block take rows in turn.
+// first of theirs.
 template <int RT>
 __global__ void __launch_bounds__(256) tree_tc_combine_kernel(const TreeParams p) {
-    pdl_wait();
     pdl_trigger();
+    // lengths come from before the attention kernel, which has waited for them: where the cut lies is found while it
+    // still runs
     const int lane = threadIdx.x & 31, warp = threadIdx.x >> 5, most = gridDim.x + 1, cut = blockIdx.x + 1;
     long long total = 0;
     for (int b0 = 0; b0 < p.batch; b0 += 32) {
@@ -958,6 +989,8 @@ __global__ void __launch_bounds__(256) tree_tc_combine_kernel(const TreeParams p
         total += w;
     }
     const int g = tc_ctas(total, most);
+    // one block waits whatever its cut, so that this grid never completes before the attention kernel
+    if (cut == 1 && blockIdx.y == 0) pdl_wait();
     if (cut >= g) return;
     const long long at = total * cut / g;      // first step behind the cut
     // its sequence
@@ -991,30 +1024,56 @@ __global__ void __launch_bounds__(256) tree_tc_combine_kernel(const TreeParams p
     const int first = (int)(((start + 1) * g + total - 1) / total) - 1;
     const int last = (int)(((start + n) * g + total - 1) / total) - 1;
     if (first != cut - 1) return;              // not the pair's first cut
+    pdl_wait();
     const int kvh = pair / tiles, rt = pair - kvh * tiles;
     const float2* ml = reinterpret_cast<const float2*>(p.part_ml);
-    const int e = lane * 4;
-    for (int local = blockIdx.y * 8 + warp; local < RT; local += gridDim.y * 8) {
-        const int pr = rt * RT + local;
-        if (pr >= rows) return;
-        auto slot = [&](int c) { return (size_t)(2 * c + (c == first ? 1 : 0)) * RT + local; };
-        float M = kTreeLowest;
-        for (int c = first; c <= last; ++c) M = fmaxf(M, ml[slot(c)].x);
-        float L = 0.f;
-        float4 acc = {0.f, 0.f, 0.f, 0.f};
-#pragma unroll 4
-        for (int c = first; c <= last; ++c) {
-            const float2 x = ml[slot(c)];
-            const float w = tree_ex2(x.x - M);
-            L += x.y * w;
-            if (e < p.d) {
-                const float4 v = *reinterpret_cast<const float4*>(p.part_o + slot(c) * p.d + e);
-                acc.x += v.x * w; acc.y += v.y * w; acc.z += v.z * w; acc.w += v.w * w;
+    // four rows a warp, their loads in flight together
+    constexpr int R = 4;
+    const int local0 = (blockIdx.y * 8 + warp) * R, e = lane * 4;
+    if (rt * RT + local0 >= rows) return;
+    float M[R], L[R];
+    float4 acc[R];
+#pragma unroll
+    for (int r = 0; r < R; ++r) { M[r] = kTreeLowest; L[r] = 0.f; acc[r] = make_float4(0.f, 0.f, 0.f, 0.f); }
+    for (int c0 = first; c0 <= last; c0 += 32) {   // a lane a part
+        const bool there = c0 + lane <= last;
+        const size_t at = (size_t)(2 * (c0 + lane) + (c0 + lane == first ? 1 : 0)) * RT + local0;
+#pragma unroll
+        for (int r = 0; r < R; ++r) M[r] = fmaxf(M[r], there ? ml[at + r].x : kTreeLowest);
+    }
+#pragma unroll
+    for (int r = 0; r < R; ++r) M[r] = warp_max(M[r]);
+    for (int c0 = first; c0 <= last; c0 += 32) {
+        const bool there = c0 + lane <= last;
+        const size_t at = (size_t)(2 * (c0 + lane) + (c0 + lane == first ? 1 : 0)) * RT + local0;
+        float w[R];
+#pragma unroll
+        for (int r = 0; r < R; ++r) {
+            const float2 x = there ? ml[at + r] : make_float2(kTreeLowest, 0.f);
+            w[r] = tree_ex2(x.x - M[r]);
+            L[r] += warp_sum(x.y * w[r]);
+        }
+        const int k = min(32, last - c0 + 1);
+#pragma unroll 2
+        for (int i = 0; i < k; ++i) {
+            const size_t from = ((size_t)(2 * (c0 + i) + (c0 + i == first ? 1 : 0)) * RT + local0) * p.d + e;
+#pragma unroll
+            for (int r = 0; r < R; ++r) {
+                const float f = __shfl_sync(0xffffffffu, w[r], i);
+                if (e < p.d) {
+                    const float4 v = *reinterpret_cast<const float4*>(p.part_o + from + (size_t)r * p.d);
+                    // a row past the pair's last holds what an earlier call left: its sums are not stored
+                    acc[r].x += v.x * f; acc[r].y += v.y * f; acc[r].z += v.z * f; acc[r].w += v.w * f;
+                }
             }
         }
-        const int i = pr / p.group;
-        const size_t orow = (size_t)(row0 + i) * p.hq + (size_t)kvh * p.group + (pr - i * p.group);
-        if (e < p.d) tree_store4(p.out, p.q_type, orow * p.d + e, acc, L == 0.f ? 0.f : 1.0f / L, L == 0.f);
+    }
+#pragma unroll
+    for (int r = 0; r < R; ++r) {
+        const int pr = rt * RT + local0 + r, i = pr / p.group;
+        if (pr < rows && e < p.d)
+            tree_store4(p.out, p.q_type, ((size_t)(row0 + i) * p.hq + (size_t)kvh * p.group + (pr - i * p.group)) * p.d + e, acc[r],
+                        L[r] == 0.f ? 0.f : 1.0f / L[r], L[r] == 0.f);
     }
 }
 
@@ -1033,7 +1092,7 @@ cudaError_t tree_tc_launch_one(const TcParams& pp, int ctas, cudaStream_t st) {
     e = launch_pdl(tree_tc_kernel<D, TILES, QS, KV>, dim3(ctas), dim3(TcShape<D, TILES, QS, KV>::kThreads), bytes, st, pp);
     if (e != cudaSuccess) return e;
     if (ctas == 1) return cudaSuccess;
-    return launch_pdl(tree_tc_combine_kernel<128 * TILES>, dim3(ctas - 1, 4), dim3(256), 0, st, pp.t);
+    return launch_pdl(tree_tc_combine_kernel<128 * TILES>, dim3(ctas - 1, 4 * TILES), dim3(256), 0, st, pp.t);
 }
 
 // Row tiles a CTA: two for pairs of more than 128 rows; 8-bit pages with fp32 q
