@@ -351,3 +351,53 @@ def test_bad_page_raises_the_flag():
     case.run()
     torch.cuda.synchronize()
     assert V.page_fault_flag() == 1
+
+
+# The plan takes lengths from max_ctx, so a small case reaches the kernel for many rows through a large one,
+# which needs a page table that could hold it; what the table has past a sequence's pages is not looked at.
+MANY = 1 << 18
+
+
+def _widen_table(case, tokens):
+    extra = np.full((case.batch, max(-(-tokens // case.pt) - case.table.shape[1], 0)), -1, dtype=np.int32)
+    case.table = np.concatenate([case.table, extra], axis=1)
+
+
+@pytest.mark.parametrize("kv", ["f16", "fp8", "int8"])
+@pytest.mark.parametrize("name", ["f32", "f16", "bf16"])
+@pytest.mark.parametrize("ctx,trees,hq,hkv,d,pt", [
+    ([0, 1, 63, 64, 65, 127, 128, 129], [1, 3, 2, 5, 1, 9, 8, 9], 4, 2, 128, 16),   # 18 rows, around a step
+    ([37, 300, 0], [8, 0, 4], 32, 8, 128, 16),
+    ([129, 700], [13, 7], 16, 2, 64, 8),
+    ([1000], [33], 8, 8, 128, 16),
+    ([250, 90], [24, 17], 8, 4, 96, 24),
+    ([130], [6], 9, 3, 16, 32),
+    ([0], [64], 1, 1, 40, 16),
+    ([5000, 3], [4, 20], 6, 2, 128, 256),                                           # pages of two steps
+])
+def test_plan_for_long_contexts(kv, name, ctx, trees, hq, hkv, d, pt):
+    torch = torch_cuda()
+    if kv != "f16" and d % 16:
+        d = 48
+    case = Case(torch, np.random.default_rng(sum(ctx) + hq + d), ctx, trees, hq, hkv, d, pt, kv, name)
+    _widen_table(case, MANY)
+    case.check(case.run(max_ctx=MANY))
+
+
+@pytest.mark.parametrize("kv", ["f16", "fp8", "int8"])
+@pytest.mark.parametrize("max_ctx", [1, 70, MANY])
+def test_contexts_past_the_bound(kv, max_ctx):
+    """max_ctx sizes the plan; lengths above it cost time, not results."""
+    torch = torch_cuda()
+    for trees in ([3, 2], [20, 9]):
+        case = Case(torch, np.random.default_rng(91), [900, 130], trees, 8, 2, 128, 16, kv, "f32")
+        _widen_table(case, max_ctx)
+        case.check(case.run(max_ctx=max_ctx))
+
+
+@pytest.mark.parametrize("kv", ["f16", "fp8", "int8"])
+def test_single_long_context_few_rows(kv):
+    """More context pieces than a warp has lanes."""
+    torch = torch_cuda()
+    case = Case(torch, np.random.default_rng(93), [9001], [2], 4, 1, 128, 16, kv, "f32")
+    case.check(case.run())

@@ -8,43 +8,65 @@
 
 namespace vb200 {
 
-// One warp a (drafted token, head): out = sum_s O_s 2^(m_s - M) / sum_s l_s 2^(m_s - M), in piece order.
+// WARPS warps a (drafted token, head): out = sum_s O_s 2^(m_s - M) / sum_s l_s 2^(m_s - M), warp w
+// taking the pieces w, w + WARPS, ... in order, the warps' sums added in theirs.
+template <int WARPS>
 __global__ void __launch_bounds__(256) tree_combine_kernel(const TreeParams p) {
+    __shared__ float4 sums[WARPS > 1 ? WARPS : 1][WARPS > 1 ? 64 : 1];
+    __shared__ float lsum[WARPS];
     pdl_wait();
     pdl_trigger();
     const int b = blockIdx.y;
     int row0;
     const int drafted = tree_rows(p, b, row0);
-    const long long r = (long long)blockIdx.x * 8 + (threadIdx.x >> 5);
-    const int lane = threadIdx.x & 31;
-    if (r >= (long long)drafted * p.hq) return;
+    const int lane = threadIdx.x & 31, w = WARPS > 1 ? (int)threadIdx.x >> 5 : 0;
+    const long long r = WARPS > 1 ? (long long)blockIdx.x : (long long)blockIdx.x * 8 + (threadIdx.x >> 5);
+    if (r >= (long long)drafted * p.hq) return;   // the same for all warps of a row
     const int total = max(p.ctx_len[b], 0) + drafted;
-    const int n = (total + p.split_tokens - 1) / p.split_tokens;
+    const int n = tree_pieces(p, total);
     if (n <= 1) return;
     const size_t row = (size_t)row0 * p.hq + (size_t)r;
     const float2* ml = reinterpret_cast<const float2*>(p.part_ml) + row * p.max_splits;
     float M = kTreeLowest;
+#pragma unroll 4
     for (int s = lane; s < n; s += 32) M = fmaxf(M, ml[s].x);
     M = warp_max(M);
     const float* part = p.part_o + row * p.max_splits * p.d;
-    // 32 pieces at a time, a lane holding the weight of one; four pieces' loads in flight
+    // 32 of the warp's pieces at a time, a lane holding the weight of one; eight pieces' loads in flight
+    const int mine = (n - w + WARPS - 1) / WARPS;   // pieces of this warp
     float L = 0.f;
     float4 acc[2] = {};
-    for (int s0 = 0; s0 < n; s0 += 32) {
-        const float2 mine = s0 + lane < n ? ml[s0 + lane] : make_float2(kTreeLowest, 0.f);
-        const float w = tree_ex2(mine.x - M);
-        L += warp_sum(mine.y * w);
-        const int k = min(32, n - s0);
-#pragma unroll 4
-        for (int s = 0; s < k; ++s) {
-            const float f = __shfl_sync(0xffffffffu, w, s);
+    for (int i0 = 0; i0 < mine; i0 += 32) {
+        const float2 one = i0 + lane < mine ? ml[w + (i0 + lane) * WARPS] : make_float2(kTreeLowest, 0.f);
+        const float f_own = tree_ex2(one.x - M);
+        L += warp_sum(one.y * f_own);
+        const int k = min(32, mine - i0);
+#pragma unroll 8
+        for (int i = 0; i < k; ++i) {
+            const float f = __shfl_sync(0xffffffffu, f_own, i);
 #pragma unroll
             for (int x = 0; x < 2; ++x) {
                 const int e = lane * 4 + 128 * x;
                 if (e < p.d) {
-                    const float4 v = *reinterpret_cast<const float4*>(part + (size_t)(s0 + s) * p.d + e);
+                    const float4 v = *reinterpret_cast<const float4*>(part + (size_t)(w + (i0 + i) * WARPS) * p.d + e);
                     acc[x].x += v.x * f; acc[x].y += v.y * f; acc[x].z += v.z * f; acc[x].w += v.w * f;
                 }
+            }
+        }
+    }
+    if constexpr (WARPS > 1) {
+        sums[w][lane] = acc[0];
+        sums[w][32 + lane] = acc[1];
+        if (lane == 0) lsum[w] = L;
+        __syncthreads();
+        if (w != 0) return;
+#pragma unroll
+        for (int v = 1; v < WARPS; ++v) {
+            L += lsum[v];
+#pragma unroll
+            for (int x = 0; x < 2; ++x) {
+                const float4 o = sums[v][32 * x + lane];
+                acc[x].x += o.x; acc[x].y += o.y; acc[x].z += o.z; acc[x].w += o.w;
             }
         }
     }
@@ -70,18 +92,32 @@ static int* tree_timeout_ptr() {
     return ptr[dev];
 }
 
+// Above this many pieces eight warps join a row, else one.  4 rows a pair, 8 KV heads, one warp / eight,
+// us: 19 pieces (8 x 2048 tokens) 32 / 29, 64 pieces (1 x 8192) 35 / 20, 128 (1 x 32768) 108 / 54.
+constexpr int kCombineWide = 8;
+
 struct TreePlan {
     bool tc;
     int ctas;                                          // tcgen05 kernel
     int wr, row_tiles, split_tokens, max_splits;       // warp-MMA kernel
 };
 
-// Rows a pair has at most: its drafted tokens times the group's heads.  From 33
-// rows on the tcgen05 kernel; below, its 128-row tiles are mostly padding and the
-// warp-MMA kernel reads the cache as fast.  Heads above 128 do not fit its
-// registers (a row's output a thread), pages of other than 8 k tokens its TMA boxes.
-static bool tree_uses_tc(long long rows, size_t d, size_t page_tokens) {
-    return rows > 32 && d <= 128 && page_tokens % 8 == 0;
+// Which kernel: rows are a pair's at most, its drafted tokens times the group's
+// heads.  The warp-MMA kernel's time grows with a pair's 16-row tiles, the tcgen05
+// kernel's, whose tile is 128 rows, does not, but its first result comes later
+// (21 us a call with next to nothing to read, against 13 to 22).  So tcgen05 from
+// 17 rows on if tiles * tokens of all pairs reach 2^18, and above 64 rows, where
+// the other kernel reads the cache more than once, always.  Warp-MMA / tcgen05, us,
+// f16 pages and queries, heads of 128, 8 KV heads:
+//   16 rows:  1 x 8192 tokens  22 /  43,  16 x 2048  56 /  55,  16 x 8192  139 / 149
+//   32 rows:  1 x 8192         28 /  43,   4 x 2048  28 /  29,  16 x 1024   49 /  39
+//   64 rows:  1 x 2048         23 /  27,   4 x  512  23 /  23,  16 x 2048  102 /  56
+//  128 rows:  1 x  256         22 /  21,   4 x 1024  42 /  26,  16 x 2048  154 /  57
+// Heads above 128 do not fit the tcgen05 kernel's registers (a row's output a
+// thread), pages of other than 8 k tokens its TMA boxes.
+static bool tree_uses_tc(long long rows, double tokens, size_t d, size_t page_tokens) {
+    return d <= 128 && page_tokens % 8 == 0 &&
+           (rows > 64 || (rows > 16 && (double)((rows + 15) / 16) * tokens >= (double)(1 << 18)));
 }
 
 // Warp-MMA: rows a CTA 16, 32 or 64, the fewest that hold a pair's rows; context
@@ -90,11 +126,12 @@ static bool tree_uses_tc(long long rows, size_t d, size_t page_tokens) {
 static TreePlan tree_plan(size_t batch, size_t max_q, size_t hq, size_t hkv, size_t d, size_t page_tokens, size_t max_ctx) {
     TreePlan t = {};
     const long long rows = (long long)max_q * (long long)(hq / hkv);
-    t.tc = tree_uses_tc(rows, d, page_tokens);
+    t.tc = tree_uses_tc(rows, (double)batch * (double)hkv * (double)max_ctx, d, page_tokens);
     if (t.tc) {
-        const long long units = (long long)batch * hkv * ((rows + 127) / 128) * (((long long)max_ctx + kTcStep - 1) / kTcStep + kTcPairCost);
-        const long long most = device_sm_count();
-        t.ctas = (int)((units + 2) / 3 < most ? (units + 2) / 3 : most);
+        const double units = (double)batch * (double)hkv * (double)((rows + 127) / 128) *
+                             (double)(((long long)max_ctx + kTcStep - 1) / kTcStep + kTcPairCost);
+        const int most = device_sm_count();
+        t.ctas = units < 3.0 * most ? (int)((units + 2) / 3) : most;
         t.max_splits = 1;
         return t;
     }
@@ -259,7 +296,9 @@ extern "C" int vspec_b200_tree_attention(const VspecB200TreeAttnArgs* a, void* s
     if (e != cudaSuccess) return cuda_status(e, "tree attention launch");
     if (p.max_splits > 1) {
         const size_t per = (size_t)p.max_q * p.hq;
-        e = launch_pdl(tree_combine_kernel, dim3((unsigned)((per + 7) / 8), p.batch), dim3(256), 0, st, p);
+        e = p.max_splits > kCombineWide
+                ? launch_pdl(tree_combine_kernel<8>, dim3((unsigned)per, p.batch), dim3(256), 0, st, p)
+                : launch_pdl(tree_combine_kernel<1>, dim3((unsigned)((per + 7) / 8), p.batch), dim3(256), 0, st, p);
         if (e != cudaSuccess) return cuda_status(e, "tree attention combine launch");
     }
     return VSPEC_B200_OK;

@@ -49,6 +49,11 @@ __device__ __forceinline__ int tree_rows(const TreeParams& p, int b, int& row0) 
     return row0 < 0 || row0 >= end ? 0 : min(end - row0, p.max_q);
 }
 
+// Context pieces of a sequence (warp-MMA kernel); the last takes what is left, also past the caller's max_ctx.
+__device__ __forceinline__ int tree_pieces(const TreeParams& p, int total) {
+    return min((total + p.split_tokens - 1) / p.split_tokens, p.max_splits);
+}
+
 // N (2, 4 or 8) consecutive values of q from each of R places (multiples of N), 0
 // where at[r] is kTreeNone.  Every load is issued whatever its place, so that all
 // of them are in flight at once: a branch around each made them wait for one

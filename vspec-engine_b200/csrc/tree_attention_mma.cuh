@@ -104,9 +104,9 @@ __global__ void __launch_bounds__(kTreeThreads) tree_mma_kernel(const TreeParams
     const int ctx = max(p.ctx_len[b], 0);
     const int total = ctx + drafted;
     const int t_begin = split * p.split_tokens;
-    if (t_begin >= total) return;
-    const int t_end = min(total, t_begin + p.split_tokens);
-    const int nsplit = (total + p.split_tokens - 1) / p.split_tokens;
+    if (t_begin >= total) return;                   // gridDim.x is max_splits
+    const int nsplit = tree_pieces(p, total);
+    const int t_end = split + 1 == nsplit ? total : t_begin + p.split_tokens;
     const int tid = threadIdx.x, warp = tid >> 5, lane = tid & 31;
     const int g = lane >> 2, c = lane & 3;
     const int wr = warp % WR, wt = warp / WR;
