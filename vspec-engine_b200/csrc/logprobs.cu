@@ -21,7 +21,6 @@ namespace vb200 {
 constexpr int kLpThreads = 256;
 constexpr int kLpWarps = kLpThreads / 32;
 constexpr int kLpMaxTop = 32;
-constexpr int kLpCandidates = 2048;
 constexpr int kLpMaxSplitRows = 2048;              // rows above this are never split
 constexpr size_t kLpCounterBytes = kLpMaxSplitRows * sizeof(unsigned);
 constexpr float kLpLowest = -3.402823466e+38f;
@@ -49,6 +48,28 @@ __device__ __forceinline__ float ex2_approx(float x) {
 __device__ __forceinline__ float max_nan(float a, float b) {
     float y;
     asm("max.NaN.f32 %0, %1, %2;" : "=f"(y) : "f"(a), "f"(b));
+    return y;
+}
+
+// Two fp32 values an instruction, each rounded as by itself.
+__device__ __forceinline__ unsigned long long pack2(float a, float b) {
+    return ((unsigned long long)__float_as_uint(b) << 32) | __float_as_uint(a);
+}
+__device__ __forceinline__ float low2(unsigned long long v) { return __uint_as_float((unsigned)v); }
+__device__ __forceinline__ float high2(unsigned long long v) { return __uint_as_float((unsigned)(v >> 32)); }
+__device__ __forceinline__ unsigned long long add2(unsigned long long a, unsigned long long b) {
+    unsigned long long y;
+    asm("add.rn.f32x2 %0, %1, %2;" : "=l"(y) : "l"(a), "l"(b));
+    return y;
+}
+__device__ __forceinline__ unsigned long long mul2(unsigned long long a, unsigned long long b) {
+    unsigned long long y;
+    asm("mul.rn.f32x2 %0, %1, %2;" : "=l"(y) : "l"(a), "l"(b));
+    return y;
+}
+__device__ __forceinline__ unsigned long long fma2(unsigned long long a, unsigned long long b, unsigned long long c) {
+    unsigned long long y;
+    asm("fma.rn.f32x2 %0, %1, %2, %3;" : "=l"(y) : "l"(a), "l"(b), "l"(c));
     return y;
 }
 
@@ -99,10 +120,9 @@ __device__ __forceinline__ unsigned long long lp_warp_sort(unsigned long long k,
 struct LpShared {
     unsigned long long lists[kLpWarps][32];   // the warps' sorted keys of a selection
     unsigned long long top[kLpMaxTop];        // the best so far, in order
-    unsigned long long bound[kLpMaxTop];      // the best of the threads' maxima
-    unsigned long long cand[kLpCandidates];
     LpStats stats[kLpWarps];
-    int count, last;
+    unsigned jth[kLpWarps];                   // ordered bits of each warp's j-th best so far, 0 = fewer
+    int last;
 };
 
 // The larger half of two ordered lists of 32, in order again: the pairs (i, 31 - i) leave a bitonic sequence.
@@ -116,12 +136,26 @@ __device__ __forceinline__ unsigned long long lp_warp_merge(unsigned long long a
     return k;
 }
 
-// out[0..32) = the largest of the CTA's keys (one a thread, 0 = none), in
-// order: every warp sorts its own, then the lists join in pairs.  Called by all
-// threads; 1 + log2(warps) barriers and one behind.
-__device__ __noinline__ void lp_select(LpShared& sm, unsigned long long key, unsigned long long* out) {
+// Lane i's key of the 32 largest of an ordered list and the keys of the lanes in `has`.
+constexpr int kLpOneByOne = 6;   // an insertion is about 15 instructions, a sort with its merge about 160
+__device__ __forceinline__ unsigned long long lp_insert(unsigned long long best, unsigned long long key, unsigned has, int lane) {
+    if (__popc(has) > kLpOneByOne) {
+        key = lp_warp_sort((has >> lane) & 1u ? key : 0ull, lane);
+        return lp_warp_merge(best, __shfl_sync(0xffffffffu, key, 31 - lane), lane);
+    }
+    for (; has; has &= has - 1) {
+        const unsigned long long k = __shfl_sync(0xffffffffu, key, __ffs(has) - 1);
+        const unsigned long long up = __shfl_up_sync(0xffffffffu, best, 1);
+        best = best > k ? best : (lane == 0 || up > k ? k : up);
+    }
+    return best;
+}
+
+// out[0..32) = the 32 largest of the warps' ordered lists (a key a lane), in
+// order; the lists join in pairs.  Called by all threads; 1 + log2(warps)
+// barriers.
+__device__ __noinline__ void lp_join_lists(LpShared& sm, unsigned long long key, unsigned long long* out) {
     const int warp = threadIdx.x >> 5, lane = threadIdx.x & 31;
-    key = lp_warp_sort(key, lane);
     sm.lists[warp][lane] = key;
 #pragma unroll 1
     for (int n = kLpWarps / 2; n > 0; n >>= 1) {
@@ -142,7 +176,7 @@ __device__ __forceinline__ void lp_take_keys(LpShared& sm, int n, Load load) {
     for (int at = 0; at < n; at += kFresh) {
         const int i = at + (int)threadIdx.x - kLpMaxTop;
         const unsigned long long key = threadIdx.x < kLpMaxTop ? sm.top[threadIdx.x] : (i < n ? load(i) : 0ull);
-        lp_select(sm, key, sm.top);
+        lp_join_lists(sm, lp_warp_sort(key, threadIdx.x & 31), sm.top);
     }
 }
 
@@ -169,36 +203,33 @@ __device__ __forceinline__ LpStats lp_join_cta(LpShared& sm, LpStats st, float c
     return st;
 }
 
-// A CTA walks over its part of a row in blocks of kLpThreads * U vectors, one
-// barrier a block, with the next block's loads in flight.  Values at or above
-// the threshold go to a candidate list; when more than 32 threads hold one (the
-// first block, rows that rise), the threshold is first raised to the top_k-th
-// largest of the threads' maxima, below which no value can be among the best.
-// At most 32 threads (top_k <= 32) then add their U * V values.
+// A CTA walks over its part of a row in blocks of kLpThreads * U vectors, with
+// the next block's loads in flight.  No warp waits for another on the way: each
+// keeps the 32 best of its own values, ordered over its lanes, and looks again
+// only at those that reach its threshold: the top_k-th of them (before there are
+// that many, the top_k-th of its lanes' maxima) or, if higher, the lowest of the
+// warps' j-th best with j * warps >= top_k.  What a warp sees of the others
+// changes its work, not what is among the best.
 template <typename T, int V, bool ALLOWED, bool TOP>
 __global__ void __launch_bounds__(kLpThreads, 4) logprobs_kernel(const LpParams p) {
     pdl_wait();
     pdl_trigger();
     constexpr int U = 16 / V;   // vectors a thread and block (16 values: more spill)
-    static_assert(32 + 32 * U * V <= kLpCandidates, "candidate list");
     const size_t row = blockIdx.y;
     const int tid = threadIdx.x, lane = tid & 31;
     const T* x = (const T*)p.logits + row * p.row_stride;
     const uint32_t* bits = ALLOWED ? p.allowed + row * p.words : nullptr;
     __shared__ LpShared sm;
     if (TOP) {
-        if (tid < kLpMaxTop) sm.top[tid] = 0;
-        if (tid == 0) sm.count = 0;
+        if (tid < kLpWarps) sm.jth[tid] = 0;
+        __syncthreads();
     }
 
     const float c = p.inv_t * 1.4426950408889634f;
     LpStats st = {kLpLowest, 0.f, 0.f};
-    unsigned long long thr = 0;   // the same in every thread
-    float thr_v = -INFINITY;
-    int pending = 32;   // the list holds no more candidates than this
-    // Draining raises the threshold to what all values so far allow; after 4, 16, ... blocks with candidates its cost
-    // (a selection, about two blocks' work) buys blocks in which fewer warps have any.
-    int offers = 0, next_drain = 4;
+    unsigned long long best = 0;   // the warp's best, in order over its lanes
+    const int j_lane = (p.top_k + kLpWarps - 1) / kLpWarps - 1;
+    float thr = kLpLowest;         // no lower value is among the row's best, the same in the warp's lanes
 
     const int j0 = blockIdx.x * p.chunk, j1 = min(p.vocab, j0 + p.chunk);
     // values before the first 16-byte boundary, whole vectors, values after the last
@@ -236,50 +267,20 @@ __global__ void __launch_bounds__(kLpThreads, 4) logprobs_kernel(const LpParams 
             st.m = top;
         }
     };
-    auto drain = [&]() {   // candidates into the list of the best
-        const int n = sm.count;
-        lp_take_keys(sm, n, [&](int i) { return sm.cand[i]; });
-        if (tid == 0) sm.count = 0;
-        __syncthreads();
-        const unsigned long long k = sm.top[p.top_k - 1];
-        if (k > thr) { thr = k; thr_v = lp_key_value(k); }
-    };
-    // candidates of a block: for_each(f, bound) calls f with the values and ids of this thread's vectors that reach
-    // the bound
-    auto offer = [&](float top, auto for_each) {
-        const int n = __syncthreads_count(top >= thr_v && top > -INFINITY);
-        if (n == 0) return;
-        // room for what this block may add, from a bound that every thread holds
-        const int most = (n > 32 ? 32 : n) * (U * V);
-        if (pending + most > kLpCandidates || ++offers == next_drain) {
-            drain();
-            pending = 0;
-            offers = 0;
-            next_drain *= 4;
-        }
-        pending += most;
-        if (n > 32) {
-            unsigned long long best = 0;
-            for_each([&](float v, int id) {
-                const unsigned long long k = v > -INFINITY ? lp_key(v, id) : 0ull;
-                best = k > best ? k : best;
-            }, -INFINITY);
-            lp_select(sm, best, sm.bound);
-            const unsigned long long k = sm.bound[p.top_k - 1];
-            if (k > thr) { thr = k; thr_v = lp_key_value(k); }
-        }
-        if (top >= thr_v)
-            for_each([&](float v, int id) {
-                // NaN fails the comparison; -inf has no place in the list
-                if (v >= thr_v && v > -INFINITY) {
-                    const unsigned long long k = lp_key(v, id);
-                    if (k >= thr) sm.cand[atomicAdd(&sm.count, 1)] = k;
-                }
-            }, thr_v);
+    auto keep = [&](float v, int id, bool want) {   // called by whole warps
+        const unsigned has = __ballot_sync(0xffffffffu, want && v >= thr);   // false for -inf and NaN
+        best = lp_insert(best, lp_key(v, id), has, lane);
+        const unsigned long long k = __shfl_sync(0xffffffffu, best, p.top_k - 1);
+        if (k) thr = fmaxf(thr, lp_key_value(k));
     };
 
     W cur[U], nxt[U];
     auto fetch = [&](int g0, W (&w)[U]) {
+        if (g0 + kLpThreads * U <= vecs) {   // no branch between the loads: all of them in flight
+#pragma unroll
+            for (int i = 0; i < U; ++i) w[i] = *reinterpret_cast<const W*>(x + body + (size_t)(g0 + i * kLpThreads + tid) * V);
+            return;
+        }
 #pragma unroll
         for (int i = 0; i < U; ++i) {
             const int g = g0 + i * kLpThreads + tid;
@@ -300,46 +301,88 @@ __global__ void __launch_bounds__(kLpThreads, 4) logprobs_kernel(const LpParams 
         if (in && (allowed_bits(j, 1) & 1u)) v = elem_to_f32<T>(x[j]);
         grow(v);
         add(v);
-        if (TOP) {
-            __syncthreads();
-            // at most 30 candidates; the threshold is still open
-            if (v > -INFINITY) sm.cand[atomicAdd(&sm.count, 1)] = lp_key(v, j);
-        }
+        if (TOP && tid < 32) keep(v, j, in);
     }
     for (int g0 = 0; g0 < vecs; g0 += kLpThreads * U) {
         fetch(g0 + kLpThreads * U, nxt);
         uint32_t ok[U];
-        float top = -INFINITY, vec_top[U];
+        float top = -INFINITY;
 #pragma unroll
         for (int i = 0; i < U; ++i) {
             const int g = g0 + i * kLpThreads + tid;
             ok[i] = ALLOWED && g < vecs ? allowed_bits(body + g * V, V) : 0u;
-            vec_top[i] = -INFINITY;
 #pragma unroll
-            for (int e = 0; e < V; ++e) vec_top[i] = fmaxf(vec_top[i], value(cur[i], e, ok[i]));
-            top = fmaxf(top, vec_top[i]);
+            for (int e = 0; e < V; ++e) top = fmaxf(top, value(cur[i], e, ok[i]));
         }
         grow(top);
+        // in pairs and without add's guard for -inf, which shows as 0 * inf in the sum; then once more with it (masks
+        // are full of -inf: at once)
+        bool guard = ALLOWED;
+        if (!ALLOWED) {
+            const unsigned long long m2 = pack2(-st.m, -st.m), c2 = pack2(c, c);
+            unsigned long long s2 = 0, u2 = 0;
 #pragma unroll
-        for (int i = 0; i < U; ++i)
+            for (int i = 0; i < U; ++i)
 #pragma unroll
-            for (int e = 0; e < V; ++e) add(value(cur[i], e, ok[i]));
-        if (TOP)
-            offer(top, [&](auto f, float bound) {
-#pragma unroll
-                for (int i = 0; i < U; ++i) {
-                    if (vec_top[i] < bound) continue;
-#pragma unroll
-                    for (int e = 0; e < V; ++e)
-                        f(value(cur[i], e, ok[i]), body + (g0 + i * kLpThreads + tid) * V + e);
+                for (int e = 0; e < V; e += 2) {
+                    const unsigned long long d = add2(pack2(value(cur[i], e, 0), value(cur[i], e + 1, 0)), m2), t = mul2(d, c2);
+                    const unsigned long long w = pack2(ex2_approx(low2(t)), ex2_approx(high2(t)));
+                    s2 = add2(s2, w);
+                    u2 = fma2(w, d, u2);
                 }
-            });
+            const float u = low2(u2) + high2(u2);
+            guard = u != u;
+            if (!guard) {
+                st.s += low2(s2) + high2(s2);
+                st.u += u;
+            }
+        }
+        if (guard) {
+#pragma unroll
+            for (int i = 0; i < U; ++i)
+#pragma unroll
+                for (int e = 0; e < V; ++e) add(value(cur[i], e, ok[i]));
+        }
+        if (TOP) {
+            const unsigned seen = __reduce_min_sync(0xffffffffu, *(volatile unsigned*)&sm.jth[lane % kLpWarps]);
+            if (seen) thr = fmaxf(thr, lp_key_value((unsigned long long)seen << 32));
+            const int n = __popc(__ballot_sync(0xffffffffu, top >= thr));
+            if (n) {
+                if (n > p.top_k && n > kLpOneByOne) {
+                    float t = top;
+#pragma unroll
+                    for (int size = 2; size <= 32; size <<= 1)
+#pragma unroll
+                        for (int o = size >> 1; o > 0; o >>= 1) {
+                            const float q = __shfl_xor_sync(0xffffffffu, t, o);
+                            t = ((lane & o) == 0) == ((lane & size) == 0) ? fmaxf(t, q) : fminf(t, q);
+                        }
+                    thr = fmaxf(thr, __shfl_sync(0xffffffffu, t, p.top_k - 1));
+                }
+                uint32_t mine = 0;
+#pragma unroll
+                for (int i = 0; i < U; ++i)
+#pragma unroll
+                    for (int e = 0; e < V; ++e) mine |= (value(cur[i], e, ok[i]) >= thr ? 1u : 0u) << (i * V + e);
+                while (__any_sync(0xffffffffu, mine != 0)) {
+                    const int at = __ffs(mine) - 1;   // -1: this lane has none left
+                    float v = 0.f;
+#pragma unroll
+                    for (int i = 0; i < U; ++i)
+#pragma unroll
+                        for (int e = 0; e < V; ++e) v = at == i * V + e ? elem_to_f32<T>(cur[i].e[e]) : v;
+                    keep(v, body + (g0 + (at / V) * kLpThreads + tid) * V + at % V, mine != 0);
+                    mine &= mine - 1;
+                }
+                if (lane == j_lane) *(volatile unsigned*)&sm.jth[tid >> 5] = (unsigned)(best >> 32);
+            }
+        }
 #pragma unroll
         for (int i = 0; i < U; ++i) cur[i] = nxt[i];
     }
 
-    st = lp_join_cta(sm, st, c);   // its barriers close the candidate list
-    if (TOP) drain();
+    st = lp_join_cta(sm, st, c);
+    if (TOP) lp_join_lists(sm, best, sm.top);
 
     if (p.splits > 1) {
         const size_t at = row * p.splits + blockIdx.x;
