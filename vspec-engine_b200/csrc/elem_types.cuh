@@ -35,4 +35,30 @@ inline int elem_vec(uintptr_t addresses, size_t counts) {
 inline bool elem_type_known(int t) { return t == VSPEC_B200_T_F32 || t == VSPEC_B200_T_F16 || t == VSPEC_B200_T_BF16; }
 
 
+// Two fp32 values an instruction, each rounded as by itself.
+typedef unsigned long long pair32;
+__device__ __forceinline__ pair32 pack2(float a, float b) {
+    pair32 y;
+    asm("mov.b64 %0, {%1, %2};" : "=l"(y) : "f"(a), "f"(b));
+    return y;
+}
+__device__ __forceinline__ void unpack2(pair32 v, float& a, float& b) { asm("mov.b64 {%0, %1}, %2;" : "=f"(a), "=f"(b) : "l"(v)); }
+__device__ __forceinline__ float low2(pair32 v) { return __uint_as_float((unsigned)v); }
+__device__ __forceinline__ float high2(pair32 v) { return __uint_as_float((unsigned)(v >> 32)); }
+__device__ __forceinline__ pair32 add2(pair32 a, pair32 b) {
+    pair32 y;
+    asm("add.rn.f32x2 %0, %1, %2;" : "=l"(y) : "l"(a), "l"(b));
+    return y;
+}
+__device__ __forceinline__ pair32 mul2(pair32 a, pair32 b) {
+    pair32 y;
+    asm("mul.rn.f32x2 %0, %1, %2;" : "=l"(y) : "l"(a), "l"(b));
+    return y;
+}
+__device__ __forceinline__ pair32 fma2(pair32 a, pair32 b, pair32 c) {
+    pair32 y;
+    asm("fma.rn.f32x2 %0, %1, %2, %3;" : "=l"(y) : "l"(a), "l"(b), "l"(c));
+    return y;
+}
+
 }  // namespace vb200

@@ -51,28 +51,6 @@ __device__ __forceinline__ float max_nan(float a, float b) {
     return y;
 }
 
-// Two fp32 values an instruction, each rounded as by itself.
-__device__ __forceinline__ unsigned long long pack2(float a, float b) {
-    return ((unsigned long long)__float_as_uint(b) << 32) | __float_as_uint(a);
-}
-__device__ __forceinline__ float low2(unsigned long long v) { return __uint_as_float((unsigned)v); }
-__device__ __forceinline__ float high2(unsigned long long v) { return __uint_as_float((unsigned)(v >> 32)); }
-__device__ __forceinline__ unsigned long long add2(unsigned long long a, unsigned long long b) {
-    unsigned long long y;
-    asm("add.rn.f32x2 %0, %1, %2;" : "=l"(y) : "l"(a), "l"(b));
-    return y;
-}
-__device__ __forceinline__ unsigned long long mul2(unsigned long long a, unsigned long long b) {
-    unsigned long long y;
-    asm("mul.rn.f32x2 %0, %1, %2;" : "=l"(y) : "l"(a), "l"(b));
-    return y;
-}
-__device__ __forceinline__ unsigned long long fma2(unsigned long long a, unsigned long long b, unsigned long long c) {
-    unsigned long long y;
-    asm("fma.rn.f32x2 %0, %1, %2, %3;" : "=l"(y) : "l"(a), "l"(b), "l"(c));
-    return y;
-}
-
 // 0 is the key of nothing: -inf and NaN have no key.
 __device__ __forceinline__ unsigned long long lp_key(float v, int id) {
     const uint32_t u = __float_as_uint(v + 0.0f);   // -0 and +0 tie
@@ -319,14 +297,14 @@ __global__ void __launch_bounds__(kLpThreads, 4) logprobs_kernel(const LpParams 
         // are full of -inf: at once)
         bool guard = ALLOWED;
         if (!ALLOWED) {
-            const unsigned long long m2 = pack2(-st.m, -st.m), c2 = pack2(c, c);
-            unsigned long long s2 = 0, u2 = 0;
+            const pair32 m2 = pack2(-st.m, -st.m), c2 = pack2(c, c);
+            pair32 s2 = 0, u2 = 0;
 #pragma unroll
             for (int i = 0; i < U; ++i)
 #pragma unroll
                 for (int e = 0; e < V; e += 2) {
-                    const unsigned long long d = add2(pack2(value(cur[i], e, 0), value(cur[i], e + 1, 0)), m2), t = mul2(d, c2);
-                    const unsigned long long w = pack2(ex2_approx(low2(t)), ex2_approx(high2(t)));
+                    const pair32 d = add2(pack2(value(cur[i], e, 0), value(cur[i], e + 1, 0)), m2), t = mul2(d, c2);
+                    const pair32 w = pack2(ex2_approx(low2(t)), ex2_approx(high2(t)));
                     s2 = add2(s2, w);
                     u2 = fma2(w, d, u2);
                 }

@@ -162,7 +162,8 @@ __device__ __forceinline__ void tc_scale(float (&v)[16], const float* s) {
 #pragma unroll
     for (int x = 0; ON && x < 16; x += 4) {
         const float4 k = *reinterpret_cast<const float4*>(s + x);
-        v[x] *= k.x; v[x + 1] *= k.y; v[x + 2] *= k.z; v[x + 3] *= k.w;
+        unpack2(mul2(pack2(v[x], v[x + 1]), pack2(k.x, k.y)), v[x], v[x + 1]);
+        unpack2(mul2(pack2(v[x + 2], v[x + 3]), pack2(k.z, k.w)), v[x + 2], v[x + 3]);
     }
 }
 
@@ -777,7 +778,10 @@ __global__ void __launch_bounds__(TcShape<D, TILES, QS, KV>::kThreads, 1) tree_t
                 const int tag = k_steps + j + 1;
                 tc_sweep<OD / 16, true>(tmem + lanes + 256u + 128u * u + (uint32_t)dim0, [&](int c, float (&v)[16]) {
 #pragma unroll
-                    for (int i = 0; i < 16; ++i) o[16 * c + i] = fmaf(o[16 * c + i], f, v[i]);
+                    for (int i = 0; i < 16; i += 2) {
+                        float* a = o + 16 * c + i;
+                        unpack2(fma2(pack2(a[0], a[1]), pack2(f, f), pack2(v[i], v[i + 1])), a[0], a[1]);
+                    }
                 });
                 if (sm.odd[(tag - 1) & 7] == tag) {
                     // infinities and NaN among the step's drafted tokens, for the rows that see them
@@ -870,13 +874,17 @@ __global__ void __launch_bounds__(TcShape<D, TILES, QS, KV>::kThreads, 1) tree_t
                 if (even) f_even = f; else f_odd = f;
                 // ---- weights 2^(s - m + 14 - v_exp), over S: 16 tokens at a time ----
                 const float bias = (KV == kTreeF16 ? 14.f : (float)(14 - v_exp)) - m_new;
-                float ls[4] = {0.f, 0.f, 0.f, 0.f};
+                pair32 ls[2] = {0, 0};
                 tc_sweep<NC, false>(s_addr, [&](int c, float (&v)[16]) {
                     tc_scale<KV != kTreeF16>(v, ks + 16 * c);
 #pragma unroll
-                    for (int x = 0; x < 16; ++x) v[x] = tree_ex2(fmaf(v[x], mul, bias));
-#pragma unroll
-                    for (int x = 0; x < 16; ++x) ls[x & 3] += v[x];
+                    for (int x = 0; x < 16; x += 2) {
+                        float a, b;
+                        unpack2(fma2(pack2(v[x], v[x + 1]), pack2(mul, mul), pack2(bias, bias)), a, b);
+                        v[x] = tree_ex2(a);
+                        v[x + 1] = tree_ex2(b);
+                        ls[(x >> 1) & 1] = add2(ls[(x >> 1) & 1], pack2(v[x], v[x + 1]));
+                    }
                     tc_scale<KV != kTreeF16>(v, &sc.v[e4][col0 + 16 * c]);
                     uint32_t h[8];
 #pragma unroll
@@ -888,7 +896,9 @@ __global__ void __launch_bounds__(TcShape<D, TILES, QS, KV>::kThreads, 1) tree_t
 #pragma unroll
                         for (int x = 0; x < 8; ++x) {
                             const float2 y = tree_unpack(h[x]);
-                            h[x] = tree_pack(v[2 * x] - y.x, v[2 * x + 1] - y.y);
+                            float a, b;
+                            unpack2(add2(pack2(v[2 * x], v[2 * x + 1]), pack2(-y.x, -y.y)), a, b);
+                            h[x] = tree_pack(a, b);
                         }
                         tc_st_x8(to + 8u, h);
                     }
@@ -898,7 +908,7 @@ __global__ void __launch_bounds__(TcShape<D, TILES, QS, KV>::kThreads, 1) tree_t
                         mbar_arrive((TILES == 2 ? c == 3 : w == 0) ? &sm.p_half[u] : &sm.p_full[u]);
                     }
                 });
-                l = fmaf(l, f, (ls[0] + ls[1]) + (ls[2] + ls[3]));
+                l = fmaf(l, f, (low2(ls[0]) + high2(ls[0])) + (low2(ls[1]) + high2(ls[1])));
                 if (KV != kTreeF16) {
                     __syncwarp();
                     if (lane == 0) mbar_arrive(&sm.sc_empty[e4]);
