@@ -435,7 +435,8 @@ typedef struct VspecB200TreeAttnArgs {
     void* d_out;                  /* [total_q][num_q_heads][head_dim], q_dtype */
     size_t batch, total_q, max_q, num_q_heads, num_kv_heads, head_dim;
     size_t page_tokens, max_pages_per_seq, num_pages;
-    size_t max_ctx;               /* host-side upper bound of ctx_len + drafted; 0 = the page table's capacity */
+    size_t max_ctx;               /* host-side upper bound of ctx_len + drafted, for the plan (longer
+                                     sequences cost time, not results); 0 = the page table's capacity */
     size_t mask_words;            /* >= ceil(max_q / 32) */
     size_t q_stride;              /* elements between rows of q; 0 = num_q_heads * head_dim */
     float scale;
