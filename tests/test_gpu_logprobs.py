@@ -209,3 +209,18 @@ def test_split_rows_share_a_workspace():
             assert all(np.array_equal(first[n], again[n]) for n in first)
     with pytest.raises(V.VspecB200Error, match="workspace"):
         _call(torch, x, "f32", None, 32, workspace=ws[:1024])
+
+
+def test_workspace_of_any_contents():
+    """What a caller's workspace held before does not matter."""
+    torch = torch_cuda()
+    rows, vocab, k = 3, 50001, 7
+    x = torch.randn((rows, vocab), device="cuda", generator=torch.Generator(device="cuda").manual_seed(3))
+    ws = torch.empty(V.lib.vspec_b200_logprobs_workspace_bytes(rows, vocab, k), dtype=torch.uint8, device="cuda")
+    assert ws.numel() > 0
+    expect = _call(torch, x, "f32", None, k)
+    for fill in (0xFF, 0x01, 0x00):
+        ws.fill_(fill)
+        got = _call(torch, x, "f32", None, k, workspace=ws)
+        torch.cuda.synchronize()
+        assert all(np.array_equal(got[n], expect[n]) for n in got)

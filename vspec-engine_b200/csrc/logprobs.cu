@@ -515,6 +515,8 @@ extern "C" int vspec_b200_logprobs(const VspecB200LogprobsArgs* a, void* stream)
         if (ws) {
             if (a->workspace_bytes < need) { set_error("workspace too small (%zu < %zu)", a->workspace_bytes, need); return VSPEC_B200_ERR_ARG; }
             if ((uintptr_t)ws % 16 != 0) { set_error("workspace must be 16-byte aligned"); return VSPEC_B200_ERR_ARG; }
+            // whatever used it before
+            VB_CHECK_CUDA(cudaMemsetAsync(ws, 0, a->rows * sizeof(unsigned), st));
         } else {
             ws = lp_scratch(need, st);
             if (!ws) { set_error("cannot allocate %zu bytes of scratch", need); return VSPEC_B200_ERR_NOMEM; }

@@ -521,36 +521,53 @@ __global__ void __launch_bounds__(TcShape<D, TILES, QS, KV>::kThreads, 1) tree_t
                     const unsigned char* rs = smem + S::kRawAt + raw * (kTcStep * D);
                     const int there = min(total - t0, kTcStep);
                     bool odd = false;
+                    // Pieces of 16 codes, piece i0 + x LANES to this lane: its place in the row and in the swizzle is the
+                    // same for every x.  The two halves of 64 dims lie in the same banks: lanes of the second store their
+                    // chunks in the other order, so that eight lanes cover all banks.
                     constexpr int PIECES = kTcStep * (D / 16), LANES = S::kFillers * 32, MINE = (PIECES + LANES - 1) / LANES;
-                    uint4 code[MINE];
+                    constexpr int ROWS = LANES / (D / 16);   // from x to x + 1
+                    static_assert(LANES % (D / 16) == 0 && ROWS % 8 == 0, "the same place in every round");
+                    const int i0 = (pw - 1) * 32 + lane, r0 = i0 / (D / 16), pc = i0 % (D / 16);
+                    const int h = pc >> 2, ch = (2 * pc) & 7;
+                    const unsigned char* from = rs + i0 * 16;
+                    unsigned char* first = st + h * kTcHalf + r0 * 128 + (((ch + h) ^ (r0 & 7)) << 4);
+                    unsigned char* second = st + h * kTcHalf + r0 * 128 + (((ch + 1 - h) ^ (r0 & 7)) << 4);
+                    auto widen = [&](const uint4 c, uint4& a, uint4& b) {
+                        tree_widen<KV>(h ? c.z : c.x, a.x, a.y);
+                        tree_widen<KV>(h ? c.w : c.y, a.z, a.w);
+                        tree_widen<KV>(h ? c.x : c.z, b.x, b.y);
+                        tree_widen<KV>(h ? c.y : c.w, b.z, b.w);
+                    };
+                    if (!drafted) {
+                        uint4 code[MINE];
 #pragma unroll
-                    for (int x = 0; x < MINE; ++x) {
-                        const int i = min((pw - 1) * 32 + lane + x * LANES, PIECES - 1);
-                        code[x] = *reinterpret_cast<const uint4*>(rs + i * 16);
-                    }
+                        for (int x = 0; x < MINE; ++x)
+                            if ((x + 1) * LANES <= PIECES || i0 + x * LANES < PIECES)
+                                code[x] = *reinterpret_cast<const uint4*>(from + x * LANES * 16);
 #pragma unroll
-                    for (int x = 0; x < MINE; ++x) {
-                        const int i = (pw - 1) * 32 + lane + x * LANES;
-                        if (i >= PIECES) break;
-                        const int r = i / (D / 16), pc = i % (D / 16);
-                        uint4 c = code[x];
-                        if (drafted && r >= there) c = make_uint4(0, 0, 0, 0);
-                        uint4 a, b;
-                        tree_widen<KV>(c.x, a.x, a.y);
-                        tree_widen<KV>(c.y, a.z, a.w);
-                        tree_widen<KV>(c.z, b.x, b.y);
-                        tree_widen<KV>(c.w, b.z, b.w);
-                        if (KV == kTreeFp8 && is_v && drafted && (tree_odd_chunk(a) || tree_odd_chunk(b))) {
-                            odd = true;
-                            tc_clear_odd(a);
-                            tc_clear_odd(b);
+                        for (int x = 0; x < MINE; ++x) {
+                            if ((x + 1) * LANES > PIECES && i0 + x * LANES >= PIECES) break;
+                            uint4 a, b;
+                            widen(code[x], a, b);
+                            *reinterpret_cast<uint4*>(first + x * ROWS * 128) = a;
+                            *reinterpret_cast<uint4*>(second + x * ROWS * 128) = b;
                         }
-                        // the two halves of 64 dims lie in the same banks: lanes of the second store their chunks in the
-                        // other order, so that eight lanes cover all banks
-                        const int h = pc >> 2, ch = (2 * pc) & 7;
-                        unsigned char* row = st + h * kTcHalf + r * 128;
-                        *reinterpret_cast<uint4*>(row + (((ch + h) ^ (r & 7)) << 4)) = h ? b : a;
-                        *reinterpret_cast<uint4*>(row + (((ch + 1 - h) ^ (r & 7)) << 4)) = h ? a : b;
+                    } else {
+                        // the few steps with drafted tokens: what is past the last token becomes 0, and so do V's infinities
+                        // and NaN, which are noted
+#pragma unroll 1
+                        for (int x = 0; i0 + x * LANES < PIECES; ++x) {
+                            uint4 c = *reinterpret_cast<const uint4*>(from + x * LANES * 16), a, b;
+                            if (r0 + x * ROWS >= there) c = make_uint4(0, 0, 0, 0);
+                            widen(c, a, b);
+                            if (KV == kTreeFp8 && is_v && (tree_odd_chunk(a) || tree_odd_chunk(b))) {
+                                odd = true;
+                                tc_clear_odd(a);
+                                tc_clear_odd(b);
+                            }
+                            *reinterpret_cast<uint4*>(first + x * ROWS * 128) = a;
+                            *reinterpret_cast<uint4*>(second + x * ROWS * 128) = b;
+                        }
                     }
                     if (odd) sm.odd[(k_steps + j) & 7] = k_steps + j + 1;
                     asm volatile("fence.proxy.async.shared::cta;\n" ::: "memory");
