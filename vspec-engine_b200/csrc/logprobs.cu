@@ -10,7 +10,10 @@
 // at again, which after a row's first block almost none do.
 // Bound by memory: a logit is read once.  Few rows: several CTAs share a row
 // and the last one to finish joins their parts in CTA order (no result depends
-// on the order of arrival).
+// on the order of arrival).  Measured, fp32 logits of 151936 tokens: 512 rows,
+// top 20, 62 us, 5.0 TB/s (76 % of a copy's rate; 512 rows are 3.5 a SM, so some
+// have 4 and some 3); 8 rows, top 5, 14.4 us, most of it the chain of the first
+// block's selection, the parts' way to the last CTA and its join.
 #include "elem_types.cuh"
 
 #include <math.h>

@@ -98,7 +98,7 @@ constexpr int kCombineWide = 8;
 
 struct TreePlan {
     bool tc;
-    int ctas;                                          // tcgen05 kernel
+    int ctas, pair_cost;                               // tcgen05 kernel
     int wr, row_tiles, split_tokens, max_splits;       // warp-MMA kernel
 };
 
@@ -120,16 +120,26 @@ static bool tree_uses_tc(long long rows, double tokens, size_t d, size_t page_to
            (rows > 64 || (rows > 16 && (double)((rows + 15) / 16) * tokens >= (double)(1 << 18)));
 }
 
+// What a change of pairs costs the tcgen05 kernel in its steps (q rows in, rows
+// out, an empty pipeline).  Sequences of 512..8192 tokens, 8 KV heads, us with 2 /
+// 3 / 4 / 6 / 8: 32 of 256 rows, fp32 q and fp16 pages 377 / 346 / 334 / 314 / 313,
+// fp16 q 267 / - / 241 / 226; 32 of 96 rows 196 / 185 / 179 / 179.  Steps on 8-bit
+// pages take longer: 16 of 256 rows - / 226 / 224 / 235, 8 of 64 rows (1024..6144
+// tokens) 59.1 / 57.8 / 61.2 / 60.7.
+static int tree_pair_cost(long long rows, bool f16) { return f16 ? (rows > 128 ? 6 : 4) : (rows > 128 ? 4 : 3); }
+
 // Warp-MMA: rows a CTA 16, 32 or 64, the fewest that hold a pair's rows; context
 // pieces: about four CTAs for each that is resident at once (sequences differ
 // in length), at least 128 tokens each.
-static TreePlan tree_plan(size_t batch, size_t max_q, size_t hq, size_t hkv, size_t d, size_t page_tokens, size_t max_ctx) {
+static TreePlan tree_plan(size_t batch, size_t max_q, size_t hq, size_t hkv, size_t d, size_t page_tokens, size_t max_ctx,
+                          bool f16) {
     TreePlan t = {};
     const long long rows = (long long)max_q * (long long)(hq / hkv);
     t.tc = tree_uses_tc(rows, (double)batch * (double)hkv * (double)max_ctx, d, page_tokens);
     if (t.tc) {
+        t.pair_cost = tree_pair_cost(rows, f16);
         const double units = (double)batch * (double)hkv * (double)((rows + 127) / 128) *
-                             (double)(((long long)max_ctx + kTcStep - 1) / kTcStep + kTcPairCost);
+                             (double)(((long long)max_ctx + kTcStep - 1) / kTcStep + t.pair_cost);
         const int most = device_sm_count();
         t.ctas = units < 3.0 * most ? (int)((units + 2) / 3) : most;
         t.max_splits = 1;
@@ -193,9 +203,9 @@ extern "C" size_t vspec_b200_tree_attention_workspace_bytes(size_t batch, size_t
     if (batch == 0 || max_q == 0 || hq == 0 || hkv == 0 || hq % hkv != 0 || d == 0 || max_ctx == 0 ||
         max_ctx > (size_t)INT_MAX || batch > 65535 || max_q > (size_t)INT_MAX / hq)
         return 0;
-    // the larger of the two kernels' (the page size decides between them)
-    const size_t a = tree_parts(tree_plan(batch, max_q, hq, hkv, d, 8, max_ctx), total_q, max_q, hq, hkv);
-    const size_t b = tree_parts(tree_plan(batch, max_q, hq, hkv, d, 1, max_ctx), total_q, max_q, hq, hkv);
+    // the larger of the two kernels' (the page size decides between them; fp16 pages take the most CTAs)
+    const size_t a = tree_parts(tree_plan(batch, max_q, hq, hkv, d, 8, max_ctx, true), total_q, max_q, hq, hkv);
+    const size_t b = tree_parts(tree_plan(batch, max_q, hq, hkv, d, 1, max_ctx, true), total_q, max_q, hq, hkv);
     return (a > b ? a : b) * (d + 2) * sizeof(float);
 }
 
@@ -237,7 +247,7 @@ extern "C" int vspec_b200_tree_attention(const VspecB200TreeAttnArgs* a, void* s
     if (al % 16 != 0) { set_error("q, out, pages and scales must be 16-byte aligned"); return VSPEC_B200_ERR_ARG; }
     if (a->total_q == 0) return VSPEC_B200_OK;
 
-    const TreePlan plan = tree_plan(a->batch, a->max_q, a->num_q_heads, a->num_kv_heads, a->head_dim, a->page_tokens, max_ctx);
+    const TreePlan plan = tree_plan(a->batch, a->max_q, a->num_q_heads, a->num_kv_heads, a->head_dim, a->page_tokens, max_ctx, f16);
     TreeParams p;
     memset(&p, 0, sizeof(p));
     p.q = a->d_q;
@@ -255,6 +265,7 @@ extern "C" int vspec_b200_tree_attention(const VspecB200TreeAttnArgs* a, void* s
     p.page_tokens = (int)a->page_tokens; p.max_pages = (int)a->max_pages_per_seq; p.num_pages = (int)a->num_pages;
     p.mask_words = (int)a->mask_words;
     p.split_tokens = plan.split_tokens; p.max_splits = plan.max_splits; p.row_tiles = plan.row_tiles;
+    p.pair_cost = plan.pair_cost;
     p.q_type = a->q_dtype;
     if ((size_t)p.hkv * p.row_tiles > 65535) { set_error("a size is too large"); return VSPEC_B200_ERR_ARG; }
     p.fault = attn_page_fault_device_ptr();

@@ -22,7 +22,8 @@ struct TreeParams {
     float scale;
     int batch, total_q, max_q, hq, hkv, group, d;
     int page_tokens, max_pages, num_pages, mask_words;
-    int split_tokens, max_splits, row_tiles;
+    int split_tokens, max_splits, row_tiles;   // warp-MMA kernel
+    int pair_cost;                             // tcgen05 kernel: steps' worth of time a pair takes besides its steps
     int q_type;
     int* fault;
 };

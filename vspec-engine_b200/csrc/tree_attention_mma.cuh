@@ -17,6 +17,10 @@
 // are rounded to fp16 once, 2^-12, no coarser than the output's own rounding.
 // P is kept times 2^14 (and, over 8-bit pages, times the V scale over a running
 // power of two), so that small weights stay normal.
+//
+// Bound by the latency of a short chain of loads when there is little to read:
+// 8 drafted tokens over 768, 4 heads a KV head, 10.4 us, 15 with the joining
+// kernel.  8 x 32768 tokens, 4 rows a pair: 238 us, 4.5 TB/s of fp16 pages.
 #pragma once
 
 #include "tc_primitives.cuh"
