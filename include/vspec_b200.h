@@ -316,7 +316,8 @@ int vspec_b200_paged_gather(const void* d_k_pages, const void* d_v_pages, const 
  * drafted tokens per sequence at once (no reference counterpart: its draft /
  * verify control plane calls the single-token kernels).  Element types of
  * activations and logits: fp32, fp16 or bf16; sums, softmax statistics and
- * angles are held in 32 bits, results are rounded once.  Calls that
+ * angles are held in 32 bits, results are rounded once.  Attention multiplies
+ * fp32 queries and softmax weights as two fp16 parts, 22 bits.  Calls that
  * share a workspace, the library's for a device and host thread among them,
  * must be stream-ordered; a workspace's contents do not matter.
  * ------------------------------------------------------------------------ */

@@ -1,0 +1,49 @@
+"""Tree attention at the ends of its inputs' ranges, in the kernel for few rows
+and in the one for many."""
+import numpy as np
+import pytest
+
+from gpu_util import torch_cuda
+from test_gpu_tree_attention import MANY, Case, _torch_type, _widen_table
+
+pytestmark = pytest.mark.gpu
+
+KERNELS = ["few rows", "many rows"]
+
+
+def _case(kernel, ctx, trees, kv, name, seed, hq=8, hkv=2, d=128, pt=16, **kw):
+    """A case whose plan takes the kernel: 17 to 64 rows a pair go to the one for many rows with a table that
+    could hold a long context, else to the other."""
+    torch = torch_cuda()
+    case = Case(torch, np.random.default_rng(seed), ctx, trees, hq, hkv, d, pt, kv, name, **kw)
+    rows = case.max_q * hq // hkv
+    assert 16 < rows <= 64 and -(-rows // 16) * case.batch * hkv * case.max_ctx < 1 << 18
+    if kernel == "many rows":
+        _widen_table(case, MANY)
+        case.max_ctx = MANY
+    return case
+
+
+@pytest.mark.parametrize("kernel", KERNELS)
+@pytest.mark.parametrize("kv", ["f16", "fp8", "int8"])
+@pytest.mark.parametrize("name", ["f16", "bf16"])
+def test_results_are_rounded_once(kernel, kv, name):
+    """16-bit queries and results: the error is that of rounding the exact result, within 1.1 for the chance of
+    which values are near a tie, and what fp32 holds: weights within 2e-5 (scores within 1e-5), so a result
+    within that of sum p |v|."""
+    case = _case(kernel, [30, 9, 61, 250], [6, 8, 5, 7], kv, name, 101)
+    out = case.run().double()
+    case.torch.cuda.synchronize()
+    ref, _ = case.ref()
+    signed = case.codes[1]
+    if kv == "f16":
+        case.codes[1] = signed.abs()
+    elif kv == "fp8":
+        case.codes[1] = signed & 0x7F
+    else:
+        case.codes[1] = signed.view(case.torch.int8).abs().view(case.torch.uint8)
+    size, _ = case.ref()
+    once = (ref.to(_torch_type(case.torch, name)).double() - ref).norm().item()
+    err = (out - ref).norm().item()
+    print(f"{kernel} {kv} {name}: {err / ref.norm().item():.3e}, rounded once {once / ref.norm().item():.3e}")
+    assert err <= 1.1 * once + 2e-5 * size.norm().item()

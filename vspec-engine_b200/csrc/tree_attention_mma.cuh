@@ -13,10 +13,10 @@
 // Products are fp16 with fp32 accumulation.  K and V codes of every page type
 // are exact in fp16; their scales multiply scores and weights, not codes.  An
 // fp32 q row is scaled by a power of two and split into hi + lo fp16 parts (22
-// bits, two MMAs), as are the weights P then; for 16-bit q and out the weights
-// are rounded to fp16 once, 2^-12, no coarser than the output's own rounding.
-// P is kept times 2^14 (and, over 8-bit pages, times the V scale over a running
-// power of two), so that small weights stay normal.
+// bits, two MMAs), and so are the weights P for every type: one part's rounding,
+// 2^-12, would show beside that of an fp16 result (error 2.9e-4 of the result in
+// place of 2.1e-4).  P is kept times 2^14 (and, over 8-bit pages, times the V
+// scale over a running power of two), so that small weights stay normal.
 //
 // Bound by the latency of a short chain of loads when there is little to read:
 // 8 drafted tokens over 768, 4 heads a KV head, 10.4 us, 15 with the joining
@@ -33,6 +33,7 @@ namespace vb200 {
 constexpr int kTreeThreads = 128;
 constexpr int kTreeTile = 64;                      // tokens a step
 constexpr int kTreeF16 = 0, kTreeFp8 = 1, kTreeInt8 = 2;
+constexpr int kTreeParts = 2;                      // fp16 parts of a weight
 
 __device__ __forceinline__ float tree_ex2(float x) {
     float y;
@@ -413,17 +414,15 @@ __global__ void __launch_bounds__(kTreeThreads) tree_mma_kernel(const TreeParams
         // ---- O = O 2^(m-m') + P V.  A step's product starts from 0 and is added in fp32: the tensor cores cut
         //      off what their accumulator cannot hold, which over thousands of tokens would add up (6e-6 of the
         //      result at 8192 tokens, against 1e-6 this way) ----
-        uint32_t a[NT / 16][QS][4];
+        uint32_t a[NT / 16][kTreeParts][4];
 #pragma unroll
         for (int k2 = 0; k2 < NT / 16; ++k2)
 #pragma unroll
             for (int x = 0; x < 4; ++x) {
                 const float lo = s[2 * k2 + (x >> 1)][(x & 1) * 2], hi = s[2 * k2 + (x >> 1)][(x & 1) * 2 + 1];
                 a[k2][0][x] = tree_pack(lo, hi);
-                if (QS == 2) {
-                    const float2 h = tree_unpack(a[k2][0][x]);
-                    a[k2][QS - 1][x] = tree_pack(lo - h.x, hi - h.y);
-                }
+                const float2 h = tree_unpack(a[k2][0][x]);
+                a[k2][1][x] = tree_pack(lo - h.x, hi - h.y);
             }
 #pragma unroll
         for (int i2 = 0; i2 < D / 16; ++i2) {
@@ -434,7 +433,7 @@ __global__ void __launch_bounds__(kTreeThreads) tree_mma_kernel(const TreeParams
                 uint32_t vb[4];
                 tree_ldsm_t(st_v + (uint32_t)r * (D * 2) + ((uint32_t)((2 * i2 + v_hi) ^ (r & 7)) << 4), vb);
 #pragma unroll
-                for (int q = 0; q < QS; ++q) {
+                for (int q = 0; q < kTreeParts; ++q) {
                     mma_16816_f16_acc(d0, a[k2][q], vb[0], vb[1]);
                     mma_16816_f16_acc(d1, a[k2][q], vb[2], vb[3]);
                 }

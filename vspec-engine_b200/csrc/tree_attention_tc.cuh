@@ -21,8 +21,8 @@
 // The grid is persistent: all pairs' steps, laid out in a row, are cut into
 // equal runs, one a CTA, so that sequences of any lengths balance to one step.
 // A run that cuts a pair writes that part's (O, m, l); a second kernel joins
-// the parts of such pairs in order.  fp32 q and 8-bit pages are split and scaled
-// as in the warp-MMA kernels.
+// the parts of such pairs in order.  fp32 q, weights and 8-bit pages are split
+// and scaled as in the warp-MMA kernels.
 //
 // Measured, 8 KV heads of 128, 16-token pages: 32 x 64 drafted tokens, 4 query
 // heads a KV head, contexts 512..8192, fp32 q and fp16 pages 312 us: 940
@@ -627,8 +627,8 @@ __global__ void __launch_bounds__(TcShape<D, TILES, QS, KV>::kThreads, 1) tree_t
 #pragma unroll
                     for (int k1 = 0; k1 < 2; ++k1)
 #pragma unroll
-                        for (int q = 0; q < QS; ++q)
-                            tc_mma_ts(d, a + 64u * half + 8u * (QS * (2 * (k2 & 1) + k1) + q), vb + (uint32_t)(2 * k2 + k1) * TOKENS, idesc_o, k2 || k1 || q);
+                        for (int q = 0; q < kTreeParts; ++q)
+                            tc_mma_ts(d, a + 64u * half + 8u * (kTreeParts * (2 * (k2 & 1) + k1) + q), vb + (uint32_t)(2 * k2 + k1) * TOKENS, idesc_o, k2 || k1 || q);
             };
             // the two halves of a step's weights have a barrier each: one barrier's second completion would hide the first
             auto wait_p = [&](int w, int half) -> bool {
@@ -915,19 +915,17 @@ __global__ void __launch_bounds__(TcShape<D, TILES, QS, KV>::kThreads, 1) tree_t
                     uint32_t h[8];
 #pragma unroll
                     for (int x = 0; x < 8; ++x) h[x] = tree_pack(v[2 * x], v[2 * x + 1]);
-                    // 8 columns of high parts, then 8 of low parts; each half of the tokens in its own half of S
-                    const uint32_t to = s_addr + (uint32_t)((c >> 2) * 64 + (c & 3) * 8 * QS);
+                    // 8 columns of high parts, then 8 of low parts, where the 16 scores were
+                    const uint32_t to = s_addr + 16u * c;
                     tc_st_x8(to, h);
-                    if constexpr (QS == 2) {
 #pragma unroll
-                        for (int x = 0; x < 8; ++x) {
-                            const float2 y = tree_unpack(h[x]);
-                            float a, b;
-                            unpack2(add2(pack2(v[2 * x], v[2 * x + 1]), pack2(-y.x, -y.y)), a, b);
-                            h[x] = tree_pack(a, b);
-                        }
-                        tc_st_x8(to + 8u, h);
+                    for (int x = 0; x < 8; ++x) {
+                        const float2 y = tree_unpack(h[x]);
+                        float a, b;
+                        unpack2(add2(pack2(v[2 * x], v[2 * x + 1]), pack2(-y.x, -y.y)), a, b);
+                        h[x] = tree_pack(a, b);
                     }
+                    tc_st_x8(to + 8u, h);
                     if ((c & 3) == 3) {      // half of the step's weights are there
                         tmem_wait_st();
                         tc_fence_before();
