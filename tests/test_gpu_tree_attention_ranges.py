@@ -3,6 +3,7 @@ and in the one for many."""
 import numpy as np
 import pytest
 
+import vspec_b200 as V
 from gpu_util import torch_cuda
 from test_gpu_tree_attention import MANY, Case, _torch_type, _widen_table
 
@@ -47,3 +48,13 @@ def test_results_are_rounded_once(kernel, kv, name):
     err = (out - ref).norm().item()
     print(f"{kernel} {kv} {name}: {err / ref.norm().item():.3e}, rounded once {once / ref.norm().item():.3e}")
     assert err <= 1.1 * once + 2e-5 * size.norm().item()
+
+
+@pytest.mark.parametrize("name", ["f32", "bf16"])
+@pytest.mark.parametrize("ctx,n,hq,hkv,d", [([0], 900, 4, 4, 64), ([50, 200], 400, 4, 2, 128), ([13], 640, 2, 1, 128)])
+def test_long_chunks_over_fp16_pages(name, ctx, n, hq, hkv, d):
+    """A prompt's chunk over many steps of 128 tokens, each of them with drafted tokens."""
+    case = Case(torch_cuda(), np.random.default_rng(n), ctx, [n] * len(ctx), hq, hkv, d, 16, "f16", name)
+    case.causal = True
+    case.check(case.run(use_cu=False))
+    assert V.tree_attention_timeout_flag() == 0

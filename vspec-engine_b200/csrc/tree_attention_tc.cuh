@@ -429,9 +429,14 @@ __global__ void __launch_bounds__(TcShape<D, TILES, QS, KV>::kThreads, 1) tree_t
                         else if (lane == 0) mbar_arrive(&sm.full[slot]);
                     } else {
                         // V of a step with drafted tokens: what is past the last token becomes 0, and so do infinities and
-                        // NaN, which are noted
-                        if (pw == 0) issue(true, j, ring + (uint32_t)slot * S::kSlot, &sm.raw_full[0]);
+                        // NaN, which are noted.  The barrier is armed again when all three warps have seen its last phase:
+                        // one that missed a phase would wait for the wrong parity.
+                        if (pw == 0) {
+                            if (!tc_wait(&sm.raw_empty[0], raw_phase ^ 1u, abort_flag)) { ok = false; break; }
+                            issue(true, j, ring + (uint32_t)slot * S::kSlot, &sm.raw_full[0]);
+                        }
                         if (!tc_wait(&sm.raw_full[0], raw_phase, abort_flag)) { ok = false; break; }
+                        if (lane == 0) mbar_arrive(&sm.raw_empty[0]);
                         raw_phase ^= 1u;
                         unsigned char* st = smem + S::kRingAt + (uint32_t)slot * S::kSlot;
                         const int there = min(total - (t_first + j * kTcStep), kTcStep);
