@@ -505,6 +505,10 @@ int vspec_b200_debug_fail_alloc_after(int n);
  * correct.  A synchronous memset on the host's side, no kernel. */
 int vspec_b200_debug_poison_static_scratch(int byte);
 
+/* Test hook: cycles after which a wait of the tcgen05 tree attention kernel gives
+ * up, of later calls of this process (negative: the default, about two seconds). */
+int vspec_b200_debug_tree_wait_cycles(long long cycles);
+
 /* Test hook: one step of the hybrid bridge's temporal hot-column rule (the
  * selection vspec_cuda_fused_linear_hybrid_bridge makes before any device work,
  * with the same per-thread state and environment): writes the columns that

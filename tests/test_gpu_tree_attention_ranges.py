@@ -58,3 +58,27 @@ def test_long_chunks_over_fp16_pages(name, ctx, n, hq, hkv, d):
     case.causal = True
     case.check(case.run(use_cu=False))
     assert V.tree_attention_timeout_flag() == 0
+
+
+@pytest.mark.parametrize("kv", ["f16", "fp8", "int8"])
+def test_waits_that_give_up_are_told_and_leave_nothing_behind(kv):
+    """With a limit of no time a call's waits may give up at once: then the flag says so, else the result is whole.
+    The calls after it are right."""
+    torch = torch_cuda()
+    case = Case(torch, np.random.default_rng(103), [6000, 3000], [40, 33], 8, 2, 128, 16, kv, "f32")
+    expect = case.run().clone()
+    torch.cuda.synchronize()
+    assert V.tree_attention_timeout_flag() == 0
+    gave_up = 0
+    try:
+        V.check(V.lib.vspec_b200_debug_tree_wait_cycles(0))
+        for _ in range(10):
+            out = case.run()
+            torch.cuda.synchronize()
+            flag = V.tree_attention_timeout_flag()
+            assert flag or torch.equal(out, expect)
+            gave_up += flag
+    finally:
+        V.check(V.lib.vspec_b200_debug_tree_wait_cycles(-1))
+    print(f"{kv}: {gave_up} of 10 calls gave up")
+    assert torch.equal(case.run(), expect) and V.tree_attention_timeout_flag() == 0

@@ -6,6 +6,8 @@
 #include <limits.h>
 #include <string.h>
 
+#include <atomic>
+
 namespace vb200 {
 
 // WARPS warps a (drafted token, head): out = sum_s O_s 2^(m_s - M) / sum_s l_s 2^(m_s - M), warp w
@@ -164,6 +166,8 @@ static size_t tree_parts(const TreePlan& t, size_t total_q, size_t max_q, size_t
     return t.max_splits > 1 ? total_q * hq * (size_t)t.max_splits : 0;
 }
 
+static std::atomic<long long> g_tree_wait_cycles{kTcWaitCycles};
+
 // Library-managed scratch, one grow-only buffer per device and host thread.
 struct TreeScratch {
     void* ptr;
@@ -195,6 +199,12 @@ extern "C" int vspec_b200_tree_attention_timeout_flag(int* out_flag) {
     VB_CHECK_CUDA(cudaMemcpyFromSymbol(&v, g_tree_timeout, sizeof(int)));
     VB_CHECK_CUDA(cudaMemcpyToSymbol(g_tree_timeout, &zero, sizeof(int)));
     *out_flag = v;
+    return VSPEC_B200_OK;
+}
+
+// Test hook: cycles after which a wait of the tcgen05 kernel gives up (negative: the default).
+extern "C" int vspec_b200_debug_tree_wait_cycles(long long cycles) {
+    g_tree_wait_cycles = cycles < 0 ? kTcWaitCycles : cycles;
     return VSPEC_B200_OK;
 }
 
@@ -291,6 +301,7 @@ extern "C" int vspec_b200_tree_attention(const VspecB200TreeAttnArgs* a, void* s
         pp.t = p;
         pp.timeout = tree_timeout_ptr();
         if (!pp.timeout) return cuda_status(cudaGetLastError(), "timeout flag");
+        pp.wait_cycles = g_tree_wait_cycles;
         pp.box_rows = 8;   // the largest power of two that divides the page, up to a whole step
         while (pp.box_rows < kTcStep && p.page_tokens % (2 * pp.box_rows) == 0) pp.box_rows *= 2;
         int rc = tree_tc_map(&pp.k_map, p.k_pages, p, f16, pp.box_rows);

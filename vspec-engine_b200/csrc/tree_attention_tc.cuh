@@ -44,7 +44,8 @@ namespace vb200 {
 
 constexpr int kTcMmaWarp = 8, kTcFirstProducer = 9;
 constexpr int kTcStep = 128;
-constexpr long long kTcWaitCycles = 4000000000ll;
+constexpr long long kTcWaitCycles = 4000000000ll;  // about two seconds
+constexpr uint32_t kTcDrainPolls = 1000000u;       // of about a microsecond
 constexpr uint32_t kTcHalf = 128u * 128u;          // 128 rows x 64 fp16
 constexpr int kTcRawSlots = 3;
 constexpr uint32_t kTcSmemMax = 232448u;
@@ -54,6 +55,7 @@ struct TcParams {
     CUtensorMap k_map, v_map;   // [pool rows][KV heads][d], boxes of box_rows x 1 x 64 values (8-bit: x d)
     int box_rows;               // divides page_tokens and kTcStep
     int* timeout;
+    long long wait_cycles;      // after which a wait gives up
 };
 
 template <int D, int TILES, int QS, int KV>
@@ -177,17 +179,21 @@ __device__ __forceinline__ void tc_scale(float (&v)[16], const float* s) {
     }
 }
 
-// Wait bounded by time (about two seconds).
-__device__ __forceinline__ bool tc_wait_one(uint64_t* bar, uint32_t parity, volatile int* abort) {
+// When a wait gives up: the CTA's flag is set, or a number of cycles have passed.
+struct TcGiveUp {
+    volatile int* flag;
+    long long cycles;
+};
+__device__ __forceinline__ bool tc_wait_one(uint64_t* bar, uint32_t parity, const TcGiveUp& up) {
     if (mbar_try_wait(bar, parity)) return true;
     const long long start = clock64();
     while (!mbar_try_wait(bar, parity))
-        if (*abort || clock64() - start > kTcWaitCycles) return false;
+        if (*up.flag || clock64() - start > up.cycles) return false;
     return true;
 }
 // The same for a whole warp, with one answer for all its lanes.
-__device__ __forceinline__ bool tc_wait(uint64_t* bar, uint32_t parity, volatile int* abort) {
-    return __all_sync(0xffffffffu, tc_wait_one(bar, parity, abort));
+__device__ __forceinline__ bool tc_wait(uint64_t* bar, uint32_t parity, const TcGiveUp& up) {
+    return __all_sync(0xffffffffu, tc_wait_one(bar, parity, up));
 }
 
 // ---- the work: sequence b has pairs (KV head, row tile) of n steps each.  A pair also costs its q rows, its
@@ -279,7 +285,7 @@ __global__ void __launch_bounds__(TcShape<D, TILES, QS, KV>::kThreads, 1) tree_t
     static_assert(sizeof(TcMisc) % 16 == 0 && S::kMiscAt % 16 == 0, "vector reads of the scales behind");
     static_assert((TILES == 2 ? offsetof(TcMisc, row) : sizeof(TcMisc)) + (KV == kTreeF16 ? 0 : sizeof(TcScales)) <= S::kMisc, "misc area");
     const int tid = threadIdx.x, warp = tid >> 5, lane = tid & 31;
-    volatile int* abort_flag = &sm.abort;
+    const TcGiveUp give_up = {&sm.abort, pp.wait_cycles};
 
     if (tid == 0) {
         sm.abort = 0;
@@ -366,10 +372,13 @@ __global__ void __launch_bounds__(TcShape<D, TILES, QS, KV>::kThreads, 1) tree_t
         uint32_t phase = 0, raw_phase = 0;   // of the slot's next use
         bool wrapped = false;                // the ring has been filled once
         int k_steps = 0;                     // steps of the CTA's run before this segment
+        // the first warp's copies, for their end after a wait that gave up: barriers with copies (a bit each) and the
+        // parity of the last of them
+        uint32_t armed = 0, armed_phase = 0, raw_armed = 0, raw_armed_phase = 0;
         auto advance = [&]() {
             if (++slot == NS) { slot = 0; phase ^= 1u; wrapped = true; }
         };
-        auto wait_slot = [&]() -> bool { return !wrapped || tc_wait(&sm.empty[slot], phase ^ 1u, abort_flag); };
+        auto wait_slot = [&]() -> bool { return !wrapped || tc_wait(&sm.empty[slot], phase ^ 1u, give_up); };
         // load li of a segment: K or V of its step j, in the order in which the products need them
         auto decode = [&](int li, bool& is_v, int& j) {
             if (TILES == 2) { is_v = li & 1; j = li >> 1; }
@@ -422,20 +431,28 @@ __global__ void __launch_bounds__(TcShape<D, TILES, QS, KV>::kThreads, 1) tree_t
                     int j;
                     decode(li, is_v, j);
                     if (j >= seg.steps) continue;
-                    if (!wait_slot()) { ok = false; break; }
                     const bool drafted = t_first + (j + 1) * kTcStep > seg.ctx;
+                    if (pw == 0 && !wait_slot()) { ok = false; break; }
                     if (!(is_v && drafted)) {
-                        if (pw == 0) issue(is_v, j, ring + (uint32_t)slot * S::kSlot, &sm.full[slot]);
-                        else if (lane == 0) mbar_arrive(&sm.full[slot]);
+                        // the first warp arrives for all, so that the phase ends with its copies, whatever the others do
+                        if (pw == 0) {
+                            if (lane == 0) mbar_arrive_n(&sm.full[slot], S::kFillers - 1);
+                            issue(is_v, j, ring + (uint32_t)slot * S::kSlot, &sm.full[slot]);
+                            armed |= 1u << slot;
+                            armed_phase = (armed_phase & ~(1u << slot)) | (phase << slot);
+                        }
                     } else {
                         // V of a step with drafted tokens: what is past the last token becomes 0, and so do infinities and
                         // NaN, which are noted.  The barrier is armed again when all three warps have seen its last phase:
                         // one that missed a phase would wait for the wrong parity.
                         if (pw == 0) {
-                            if (!tc_wait(&sm.raw_empty[0], raw_phase ^ 1u, abort_flag)) { ok = false; break; }
+                            if (!tc_wait(&sm.raw_empty[0], raw_phase ^ 1u, give_up)) { ok = false; break; }
                             issue(true, j, ring + (uint32_t)slot * S::kSlot, &sm.raw_full[0]);
+                            raw_armed = 1u;
+                            raw_armed_phase = raw_phase;
+                            armed &= ~(1u << slot);     // the slot's last copies are these
                         }
-                        if (!tc_wait(&sm.raw_full[0], raw_phase, abort_flag)) { ok = false; break; }
+                        if (!tc_wait(&sm.raw_full[0], raw_phase, give_up)) { ok = false; break; }
                         if (lane == 0) mbar_arrive(&sm.raw_empty[0]);
                         raw_phase ^= 1u;
                         unsigned char* st = smem + S::kRingAt + (uint32_t)slot * S::kSlot;
@@ -494,12 +511,14 @@ __global__ void __launch_bounds__(TcShape<D, TILES, QS, KV>::kThreads, 1) tree_t
                         int j;
                         decode(li, is_v, j);
                         if (j >= seg.steps) continue;
-                        if (wrapped && !tc_wait(&sm.raw_empty[raw], raw_phase ^ 1u, abort_flag)) { ok = false; break; }
+                        if (wrapped && !tc_wait(&sm.raw_empty[raw], raw_phase ^ 1u, give_up)) { ok = false; break; }
                         issue(is_v, j, smem_u32(smem) + S::kRawAt + (uint32_t)raw * (kTcStep * D), &sm.raw_full[raw]);
+                        raw_armed |= 1u << raw;
+                        raw_armed_phase = (raw_armed_phase & ~(1u << raw)) | (raw_phase << raw);
                         if (++raw == kTcRawSlots) { raw = 0; raw_phase ^= 1u; wrapped = true; }
                         if (is_v) continue;
                         const int k = k_steps + j, e = k & 3;
-                        if (k >= 4 && !tc_wait(&sm.sc_empty[e], (uint32_t)((k >> 2) - 1) & 1u, abort_flag)) { ok = false; break; }
+                        if (k >= 4 && !tc_wait(&sm.sc_empty[e], (uint32_t)((k >> 2) - 1) & 1u, give_up)) { ok = false; break; }
                         const bool drafted = t_first + (j + 1) * kTcStep > seg.ctx;
                         float top = 0.f;
 #pragma unroll
@@ -530,7 +549,7 @@ __global__ void __launch_bounds__(TcShape<D, TILES, QS, KV>::kThreads, 1) tree_t
                     if (j >= seg.steps) continue;
                     const int t0 = t_first + j * kTcStep;
                     const bool drafted = t0 + kTcStep > seg.ctx;
-                    if (!tc_wait(&sm.raw_full[raw], raw_phase, abort_flag) || !wait_slot()) { ok = false; break; }
+                    if (!tc_wait(&sm.raw_full[raw], raw_phase, give_up) || !wait_slot()) { ok = false; break; }
                     unsigned char* st = smem + S::kRingAt + (uint32_t)slot * S::kSlot;
                     const unsigned char* rs = smem + S::kRawAt + raw * (kTcStep * D);
                     const int there = min(total - t0, kTcStep);
@@ -593,7 +612,15 @@ __global__ void __launch_bounds__(TcShape<D, TILES, QS, KV>::kThreads, 1) tree_t
             }
             k_steps += seg.steps;
         }
-        if (!ok) { *abort_flag = 1; atomicOr(pp.timeout, 1); }
+        if (!ok) { *give_up.flag = 1; atomicOr(pp.timeout, 1); }
+        // every copy lands before shared memory is released, also where a wait gave up
+        if (pw == 0 && lane == 0) {
+            for (int i = 0; i < NS; ++i)
+                if ((armed >> i) & 1u) (void)mbar_wait_drain(&sm.full[i], (armed_phase >> i) & 1u, kTcDrainPolls);
+            for (int i = 0; i < kTcRawSlots; ++i)
+                if ((raw_armed >> i) & 1u) (void)mbar_wait_drain(&sm.raw_full[i], (raw_armed_phase >> i) & 1u, kTcDrainPolls);
+        }
+        __syncwarp();
     } else {
         // ============================ tensor cores =========================
         if (lane == 0) {
@@ -604,7 +631,7 @@ __global__ void __launch_bounds__(TcShape<D, TILES, QS, KV>::kThreads, 1) tree_t
             uint32_t phase = 0;
             uint32_t q_phase = 0, p_phase[2] = {0, 0};
             auto take = [&](int& s) -> bool {   // next tile of the ring
-                if (!tc_wait_one(&sm.full[slot], phase, abort_flag)) return false;
+                if (!tc_wait_one(&sm.full[slot], phase, give_up)) return false;
                 s = slot;
                 if (++slot == NS) { slot = 0; phase ^= 1u; }
                 return true;
@@ -637,13 +664,13 @@ __global__ void __launch_bounds__(TcShape<D, TILES, QS, KV>::kThreads, 1) tree_t
             };
             // the two halves of a step's weights have a barrier each: one barrier's second completion would hide the first
             auto wait_p = [&](int w, int half) -> bool {
-                if (!tc_wait_one(half ? &sm.p_full[w] : &sm.p_half[w], p_phase[w], abort_flag)) return false;
+                if (!tc_wait_one(half ? &sm.p_full[w] : &sm.p_half[w], p_phase[w], give_up)) return false;
                 if (half) p_phase[w] ^= 1u;
                 tc_fence_after();
                 return true;
             };
             while (ok && walk.next(p, seg)) {
-                if (!tc_wait_one(&sm.q_full, q_phase, abort_flag)) { ok = false; break; }
+                if (!tc_wait_one(&sm.q_full, q_phase, give_up)) { ok = false; break; }
                 q_phase ^= 1u;
                 int ks = 0, vs = 0;
                 if (TILES == 2) {
@@ -690,11 +717,10 @@ __global__ void __launch_bounds__(TcShape<D, TILES, QS, KV>::kThreads, 1) tree_t
                     }
                 }
             }
-            if (!ok) { *abort_flag = 1; atomicOr(pp.timeout, 1); }
+            if (!ok) { *give_up.flag = 1; atomicOr(pp.timeout, 1); }
             // every product completes before tensor memory is released
             umma_commit(&sm.drain);
-            volatile int never = 0;
-            (void)tc_wait_one(&sm.drain, 0u, &never);
+            (void)mbar_wait_drain(&sm.drain, 0u, kTcDrainPolls);
         }
         __syncwarp();
     }
@@ -786,7 +812,7 @@ __global__ void __launch_bounds__(TcShape<D, TILES, QS, KV>::kThreads, 1) tree_t
                         for (int x = 0; x < p.d * es; x += 128) asm volatile("prefetch.global.L2 [%0];\n" ::"l"(at + x));
                     }
                 }
-                if (!tc_wait(&sm.q_full, q_phase, abort_flag)) { ok = false; break; }
+                if (!tc_wait(&sm.q_full, q_phase, give_up)) { ok = false; break; }
                 q_phase ^= 1u;
             }
             const int local = (TILES == 2 ? 128 * w : 0) + row;     // row of the tile pair
@@ -843,7 +869,7 @@ __global__ void __launch_bounds__(TcShape<D, TILES, QS, KV>::kThreads, 1) tree_t
             for (int i = 0; i < n + LAG; ++i) {
                 const int u = TILES == 2 ? w : i & 1;
                 if (i < n || i >= LAG) {
-                    if (!tc_wait(&sm.s_full[u], (s_phase >> u) & 1u, abort_flag)) { ok = false; break; }
+                    if (!tc_wait(&sm.s_full[u], (s_phase >> u) & 1u, give_up)) { ok = false; break; }
                     s_phase ^= 1u << u;
                     tc_fence_after();
                 }
@@ -853,7 +879,7 @@ __global__ void __launch_bounds__(TcShape<D, TILES, QS, KV>::kThreads, 1) tree_t
                 const uint32_t s_addr = tmem + lanes + 128u * u + (uint32_t)col0;
                 const int t0 = (seg.step0 + i) * kTcStep + col0, e4 = (k_steps + i) & 3;
                 const bool masked = (seg.step0 + i + 1) * kTcStep > seg.ctx;
-                if (KV != kTreeF16 && !tc_wait(&sm.sc_full[e4], (uint32_t)((k_steps + i) >> 2) & 1u, abort_flag)) { ok = false; break; }
+                if (KV != kTreeF16 && !tc_wait(&sm.sc_full[e4], (uint32_t)((k_steps + i) >> 2) & 1u, give_up)) { ok = false; break; }
                 const float* ks = KV == kTreeF16 ? nullptr : sc.k[e4] + col0;
                 if (masked) {
                     // what the row does not see becomes -inf in S; the scales of K are applied on the way
@@ -887,7 +913,7 @@ __global__ void __launch_bounds__(TcShape<D, TILES, QS, KV>::kThreads, 1) tree_t
                     sm.row[i & 1][w][row] = top;
                     tc_fence_before();
                     mbar_arrive(&sm.pair);
-                    if (!tc_wait(&sm.pair, pair_phase, abort_flag)) { ok = false; break; }
+                    if (!tc_wait(&sm.pair, pair_phase, give_up)) { ok = false; break; }
                     pair_phase ^= 1u;
                     tc_fence_after();
                     top = fmaxf(top, sm.row[i & 1][w ^ 1][row]);
@@ -954,7 +980,7 @@ __global__ void __launch_bounds__(TcShape<D, TILES, QS, KV>::kThreads, 1) tree_t
                 // the weights of the other group's tokens
                 sm.row[n & 1][w][row] = l;
                 mbar_arrive(&sm.pair);
-                if (!tc_wait(&sm.pair, pair_phase, abort_flag)) { ok = false; break; }
+                if (!tc_wait(&sm.pair, pair_phase, give_up)) { ok = false; break; }
                 pair_phase ^= 1u;
                 l += sm.row[n & 1][w ^ 1][row];
             }
@@ -997,11 +1023,11 @@ __global__ void __launch_bounds__(TcShape<D, TILES, QS, KV>::kThreads, 1) tree_t
             // every warp's stage has been read before any writes the next segment's q there
             uint64_t* read = TILES == 1 ? &sm.pair : &sm.staged[w];
             mbar_arrive(read);
-            if (!tc_wait(read, TILES == 1 ? pair_phase : staged_phase, abort_flag)) { ok = false; break; }
+            if (!tc_wait(read, TILES == 1 ? pair_phase : staged_phase, give_up)) { ok = false; break; }
             if (TILES == 1) pair_phase ^= 1u; else staged_phase ^= 1u;
             tc_fence_after();
         }
-        if (!ok) { *abort_flag = 1; atomicOr(pp.timeout, 1); }
+        if (!ok) { *give_up.flag = 1; atomicOr(pp.timeout, 1); }
     }
     tc_fence_before();
     __syncthreads();
