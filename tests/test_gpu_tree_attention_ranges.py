@@ -82,3 +82,22 @@ def test_waits_that_give_up_are_told_and_leave_nothing_behind(kv):
         V.check(V.lib.vspec_b200_debug_tree_wait_cycles(-1))
     print(f"{kv}: {gave_up} of 10 calls gave up")
     assert torch.equal(case.run(), expect) and V.tree_attention_timeout_flag() == 0
+
+
+def _slots(case, b, t):
+    """Pool rows of sequence b's tokens t."""
+    t = np.asarray(t)
+    return case.torch.from_numpy(case.table[b, t // case.pt].astype(np.int64) * case.pt + t % case.pt).cuda()
+
+
+@pytest.mark.parametrize("kernel", KERNELS)
+@pytest.mark.parametrize("kv", ["fp8", "int8"])
+@pytest.mark.parametrize("zeros", [(0, 128), (0, 300), (128, 1100), (0, 1999)])
+def test_v_rows_of_zeros_count_in_the_sum(kernel, kv, zeros):
+    """V rows of zeros have scale 0; their tokens weigh as much as others."""
+    case = _case(kernel, [2000, 1990, 1500, 700], [8, 5, 7, 6], kv, "f32", 104, hq=32, hkv=8)
+    for b, c in enumerate(case.ctx):
+        at = _slots(case, b, np.arange(zeros[0], min(zeros[1], c)))
+        case.codes[1][at] = 0
+        case.scales[1][at] = 0.0
+    case.check(case.run())

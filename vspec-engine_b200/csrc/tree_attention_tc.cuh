@@ -919,16 +919,17 @@ __global__ void __launch_bounds__(TcShape<D, TILES, QS, KV>::kThreads, 1) tree_t
                     top = fmaxf(top, sm.row[i & 1][w ^ 1][row]);
                 }
                 const float m_new = top == -INFINITY ? m : fmaxf(m, top * mul);
-                float f = tree_ex2(m - m_new);
+                const float f = tree_ex2(m - m_new);
+                float fo = f;                // O is kept in units of 2^v_exp, l is not
                 m = m_new;
                 if (KV != kTreeF16) {
                     const int ex = sc.v_exp[e4];
                     if (ex > v_exp) {
-                        f *= v_exp > -100 ? ldexpf(1.0f, max(v_exp - ex, -126)) : 0.f;
+                        fo *= ldexpf(1.0f, max(v_exp - ex, -126));
                         v_exp = ex;
                     }
                 }
-                if (even) f_even = f; else f_odd = f;
+                if (even) f_even = fo; else f_odd = fo;
                 // ---- weights 2^(s - m + 14 - v_exp), over S: 16 tokens at a time ----
                 const float bias = (KV == kTreeF16 ? 14.f : (float)(14 - v_exp)) - m_new;
                 pair32 ls[2] = {0, 0};
@@ -963,7 +964,8 @@ __global__ void __launch_bounds__(TcShape<D, TILES, QS, KV>::kThreads, 1) tree_t
                         mbar_arrive((TILES == 2 ? c == 3 : w == 0) ? &sm.p_half[u] : &sm.p_full[u]);
                     }
                 });
-                l = fmaf(l, f, (low2(ls[0]) + high2(ls[0])) + (low2(ls[1]) + high2(ls[1])));
+                const float sum = (low2(ls[0]) + high2(ls[0])) + (low2(ls[1]) + high2(ls[1]));
+                l = fmaf(l, f, sum * (KV == kTreeF16 ? 1.0f / kTreePScale : __uint_as_float((uint32_t)(127 + v_exp - 14) << 23)));
                 if (KV != kTreeF16) {
                     __syncwarp();
                     if (lane == 0) mbar_arrive(&sm.sc_empty[e4]);
@@ -973,7 +975,6 @@ __global__ void __launch_bounds__(TcShape<D, TILES, QS, KV>::kThreads, 1) tree_t
             k_steps += n;
             // ---- the rows: natural scale, out ----
             const float unit = ldexpf(1.0f / kTreePScale, KV == kTreeF16 ? 0 : v_exp);
-            l *= unit;
 #pragma unroll
             for (int i = 0; i < OD; ++i) o[i] *= unit;
             if (TILES == 1) {
