@@ -5,7 +5,7 @@ import pytest
 
 import vspec_b200 as V
 from gpu_util import torch_cuda
-from test_gpu_tree_attention import MANY, Case, _torch_type, _widen_table
+from test_gpu_tree_attention import BOUND, MANY, Case, _torch_type, _widen_table
 
 pytestmark = pytest.mark.gpu
 
@@ -101,3 +101,34 @@ def test_v_rows_of_zeros_count_in_the_sum(kernel, kv, zeros):
         case.codes[1][at] = 0
         case.scales[1][at] = 0.0
     case.check(case.run())
+
+
+@pytest.mark.parametrize("kernel", KERNELS)
+@pytest.mark.parametrize("kv", ["f16", "fp8", "int8"])
+@pytest.mark.parametrize("name", ["f32", "f16"])
+def test_committed_values_that_are_not_finite_reach_every_row(kernel, kv, name):
+    """NaN and infinities in V (codes or scales) of a committed token make results non-finite where the definition
+    does, also when the token shares its step with drafted ones."""
+    torch = torch_cuda()
+    for t, what in ((70, "nan"), (150, "inf"), (290, "inf"), (20, "nan")):
+        case = _case(kernel, [300, 160], [6, 7], kv, name, 105)
+        at = _slots(case, 0 if t > 160 else 1, [t])
+        value = float(what)
+        if kv == "f16":
+            case.codes[1][at, 0, 5::16] = value
+        elif kv == "fp8" and what == "nan":
+            case.codes[1][at, 0, 5::16] = 0x7F
+        else:
+            case.scales[1][at, 0] = value
+        got = case.run().double()
+        torch.cuda.synchronize()
+        ref, _ = case.ref()
+        fine = torch.isfinite(ref)
+        assert not fine.all() and fine.any()
+        if kv != "f16" and what == "inf":      # a code of 0 times the scale is NaN, any other an infinity
+            assert not torch.isfinite(got[~fine]).any()
+        else:
+            assert torch.equal(torch.isnan(got), torch.isnan(ref)) and torch.equal(torch.isinf(got), torch.isinf(ref))
+        top = float(torch.nan_to_num(torch.cat([case.rows64(1, b, c + n).flatten() for b, (c, n) in
+                                                enumerate(zip(case.ctx, case.trees))]), 0, 0, 0).abs().max())
+        assert (got - ref)[fine].abs().max().item() <= BOUND[name] * top

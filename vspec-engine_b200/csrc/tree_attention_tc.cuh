@@ -841,10 +841,11 @@ __global__ void __launch_bounds__(TcShape<D, TILES, QS, KV>::kThreads, 1) tree_t
                     }
                 });
                 if (sm.odd[(tag - 1) & 7] == tag) {
-                    // infinities and NaN among the step's drafted tokens, for the rows that see them
+                    // infinities and NaN that the producers took out of the step's V, for the rows that see them (committed
+                    // tokens: all)
                     const int32_t* table = p.table + (size_t)seg.b * p.max_pages;
                     const int t0 = (seg.step0 + j) * kTcStep;
-                    for (int t = max(t0, seg.ctx); t < min(t0 + kTcStep, seg.ctx + seg.drafted); ++t) {
+                    for (int t = t0; t < min(t0 + kTcStep, seg.ctx + seg.drafted); ++t) {
                         if (!in || !tree_sees(p, seg.row0, ti, seg.ctx, seg.drafted, t)) continue;
                         const size_t head = (size_t)tree_pool_row(p, table, t) * p.hkv + seg.kvh, at = head * p.d + dim0;
                         const float vs = KV == kTreeF16 ? 1.f : __ldg(p.v_scales + head);
