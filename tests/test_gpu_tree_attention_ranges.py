@@ -132,3 +132,35 @@ def test_committed_values_that_are_not_finite_reach_every_row(kernel, kv, name):
         top = float(torch.nan_to_num(torch.cat([case.rows64(1, b, c + n).flatten() for b, (c, n) in
                                                 enumerate(zip(case.ctx, case.trees))]), 0, 0, 0).abs().max())
         assert (got - ref)[fine].abs().max().item() <= BOUND[name] * top
+
+
+@pytest.mark.parametrize("kernel", KERNELS)
+@pytest.mark.parametrize("kv", ["fp8", "int8"])
+@pytest.mark.parametrize("name", ["f32", "f16"])
+@pytest.mark.parametrize("power", [20, 40, 60, 100])
+def test_large_v_scales_that_are_not_seen_do_not_reach_a_row(kernel, kv, name, power):
+    """V scales of drafted tokens 2^power times the others': rows that do not see them are as without them, bit
+    for bit, and rows that do are right, in a tree behind a context and in a chunk at the start of one."""
+    torch = torch_cuda()
+    for ctx, causal in (([75, 130], False), ([0, 3], True)):
+        case = _case(kernel, ctx, [12, 9], kv, name, 106)
+        case.causal = causal
+        bad = {0: [7], 1: [5, 6]}
+        if not causal:
+            for b, row in ((0, 0), (1, 12)):
+                for j in bad[b]:
+                    case.bits[row:row + case.trees[b], 0] &= ~np.uint32(1 << j)
+        clean = case.run().clone()
+        case.check(clean)
+        if not causal:
+            case.bits[3, 0] |= np.uint32(1 << 7)
+            case.bits[12 + 8, 0] |= np.uint32(1 << 5)
+        for b in bad:
+            case.scales[1][_slots(case, b, [ctx[b] + j for j in bad[b]])] *= 2.0 ** power
+        got = case.run()
+        sees = list(range(7, 12)) + list(range(12 + 5, 12 + 9)) if causal else [3, 12 + 8]
+        rest = [i for i in range(21) if i not in sees]
+        torch.cuda.synchronize()
+        assert torch.equal(got[rest], clean[rest])
+        if name == "f32":                    # fp16 results end at 65504
+            case.check(got)

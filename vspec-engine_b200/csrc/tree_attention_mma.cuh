@@ -255,7 +255,9 @@ __global__ void __launch_bounds__(kTreeThreads) tree_mma_kernel(const TreeParams
 #pragma unroll
     for (int i = 0; i < D / 8; ++i) o[i][0] = o[i][1] = o[i][2] = o[i][3] = 0.f;
     float m_run[2] = {kTreeLowest, kTreeLowest}, l_run[2] = {0.f, 0.f};
-    int v_exp = -100;                                // 8-bit pages: weights carry V scale / 2^v_exp
+    int v_exp[2] = {-100, -100};                     // 8-bit pages: a row's weights carry V scale / 2^v_exp
+    float v_mul[2];                                  // 2^(14 - v_exp)
+    v_mul[0] = v_mul[1] = KV == kTreeF16 ? kTreePScale : __uint_as_float((127u + 114u) << 23);
     const float mul0 = sm_mul[wr * 16 + g], mul1 = sm_mul[wr * 16 + g + 8];
     const int pr0 = rt * MT + wr * 16 + g, pr1 = pr0 + 8;   // rows of the pair
     const int a_row = wr * 16 + (lane & 15), a_hi = lane >> 4;
@@ -339,36 +341,51 @@ __global__ void __launch_bounds__(kTreeThreads) tree_mma_kernel(const TreeParams
         float f0 = tree_ex2(m_run[0] - n0), f1 = tree_ex2(m_run[1] - n1);
         m_run[0] = n0; m_run[1] = n1;
         l_run[0] *= f0; l_run[1] *= f1;
-        float v_mul = kTreePScale;
         if (KV != kTreeF16) {
-            const float2 vs = *reinterpret_cast<const float2*>(&sm_scale[it & 1][1][2 * lane]);
-            float top = 0.f;
-            if (vs.x <= 3.402823466e+38f) top = vs.x;
-            if (vs.y <= 3.402823466e+38f) top = fmaxf(top, vs.y);
-            top = warp_max(top);
-            int ex = -100;
-            if (top > 0.f) (void)frexpf(top, &ex);
-            if (ex > v_exp) {
-                const float f = v_exp > -100 ? ldexpf(1.0f, max(v_exp - ex, -126)) : 0.f;
-                f0 *= f; f1 *= f;                    // O so far is 0 while v_exp is at its start
-                v_exp = ex;
+            // the unit goes by what the row sees: a larger scale beside it would push its weights below fp16
+            float top[2] = {0.f, 0.f};
+            if (!masked) {
+                const float2 vs = *reinterpret_cast<const float2*>(&sm_scale[it & 1][1][2 * lane]);
+                if (vs.x <= 3.402823466e+38f) top[0] = vs.x;
+                if (vs.y <= 3.402823466e+38f) top[0] = fmaxf(top[0], vs.y);
+                top[0] = top[1] = warp_max(top[0]);
+            } else {
+#pragma unroll
+                for (int n = 0; n < NT / 8; ++n) {
+                    const float2 vs = *reinterpret_cast<const float2*>(&sm_scale[it & 1][1][wt * NT + n * 8 + 2 * c]);
+#pragma unroll
+                    for (int e = 0; e < 4; ++e) {
+                        const float v = (e & 1) ? vs.y : vs.x;
+                        if (((seen >> (4 * n + e)) & 1u) && v <= 3.402823466e+38f) top[e >> 1] = fmaxf(top[e >> 1], v);
+                    }
+                }
+#pragma unroll
+                for (int x = 1; x <= 2; x <<= 1) {
+                    top[0] = fmaxf(top[0], __shfl_xor_sync(0xffffffffu, top[0], x));
+                    top[1] = fmaxf(top[1], __shfl_xor_sync(0xffffffffu, top[1], x));
+                }
             }
-            v_mul = ldexpf(kTreePScale, -v_exp);
+#pragma unroll
+            for (int x = 0; x < 2; ++x) {
+                const int ex = max((int)(__float_as_uint(top[x]) >> 23) - 126, -100);
+                if (ex > v_exp[x]) {
+                    (x ? f1 : f0) *= __uint_as_float((uint32_t)(127 + max(v_exp[x] - ex, -126)) << 23);
+                    v_mul[x] = __uint_as_float((uint32_t)(127 + 14 - ex) << 23);
+                    v_exp[x] = ex;
+                }
+            }
         }
         // ---- weights ----
 #pragma unroll
         for (int n = 0; n < NT / 8; ++n) {
-            float w0 = v_mul, w1 = v_mul;
-            if (KV != kTreeF16) {
-                const float2 vs = *reinterpret_cast<const float2*>(&sm_scale[it & 1][1][wt * NT + n * 8 + 2 * c]);
-                w0 *= vs.x; w1 *= vs.y;
-            }
+            float2 vs = {1.f, 1.f};
+            if (KV != kTreeF16) vs = *reinterpret_cast<const float2*>(&sm_scale[it & 1][1][wt * NT + n * 8 + 2 * c]);
 #pragma unroll
             for (int e = 0; e < 4; ++e) {
                 const float x = tree_ex2(s[n][e] - (e < 2 ? n0 : n1));
                 l_run[e >> 1] += x;
                 // a weight of 0 must not meet the V scale of a token that the row does not see
-                s[n][e] = KV == kTreeF16 || ((seen >> (4 * n + e)) & 1u) ? x * ((e & 1) ? w1 : w0) : 0.f;
+                s[n][e] = KV == kTreeF16 || ((seen >> (4 * n + e)) & 1u) ? x * (v_mul[e >> 1] * ((e & 1) ? vs.y : vs.x)) : 0.f;
             }
         }
         // ---- a non-finite V among drafted tokens: its product goes to the rows that see it, and the value is
@@ -451,7 +468,9 @@ __global__ void __launch_bounds__(kTreeThreads) tree_mma_kernel(const TreeParams
     }
 
     // ---- join the token warps, write ----
-    const float unit = KV == kTreeF16 ? 1.0f / kTreePScale : ldexpf(1.0f / kTreePScale, v_exp);
+    float unit[2];
+#pragma unroll
+    for (int x = 0; x < 2; ++x) unit[x] = KV == kTreeF16 ? 1.0f / kTreePScale : ldexpf(1.0f / kTreePScale, v_exp[x]);
 #pragma unroll
     for (int x = 1; x <= 2; x <<= 1) {
         l_run[0] += __shfl_xor_sync(0xffffffffu, l_run[0], x);
@@ -469,7 +488,7 @@ __global__ void __launch_bounds__(kTreeThreads) tree_mma_kernel(const TreeParams
     for (int i = 0; i < D / 8; ++i)
 #pragma unroll
         for (int x = 0; x < 2; ++x) {
-            float2 v = {o[i][2 * x] * unit, o[i][2 * x + 1] * unit};
+            float2 v = {o[i][2 * x] * unit[x], o[i][2 * x + 1] * unit[x]};
             *reinterpret_cast<float2*>(sm_o + ((size_t)wt * MT + wr * 16 + g + 8 * x) * D + i * 8 + 2 * c) = v;
         }
     __syncthreads();

@@ -71,7 +71,7 @@ struct TcShape {
     static constexpr uint32_t kSlot = kTcStep * D * 2;
     static constexpr uint32_t kQ = TILES * QS * kSlot;
     static constexpr uint32_t kRaw = KV == kTreeF16 ? 0 : kTcRawSlots * kTcStep * D;
-    static constexpr uint32_t kMisc = KV == kTreeF16 ? (TILES == 2 ? 3072 : 4096) : 8192;
+    static constexpr uint32_t kMisc = KV == kTreeF16 ? (TILES == 2 ? 3072 : 4096) : (TILES == 2 ? 8192 : 10240);
     static constexpr int kFit = (int)((kTcSmemMax - kMisc - kQ - kRaw) / kSlot);
     static constexpr int kMost = 6;
     static constexpr int kSlots = kFit < kMost ? kFit : kMost;
@@ -89,7 +89,8 @@ struct alignas(16) TcMisc {
     int start_b;
     long long start_off, total;
     int odd[8];                 // step + 1 where V held infinities or NaN
-    float row[2][2][128];       // maxima, at last sums, of the two softmax groups (TILES = 1), in turn
+    alignas(16) float row[2][2][128];       // maxima, at last sums, of the two softmax groups (TILES = 1), in turn
+    int v_exp[2][2][128];       // exponents of the largest V scales that the groups' rows see (8-bit pages), in turn
 };
 struct alignas(16) TcScales {   // 8-bit pages: scales of four steps, read four at a time
     float k[4][kTcStep], v[4][kTcStep];
@@ -281,9 +282,11 @@ __global__ void __launch_bounds__(TcShape<D, TILES, QS, KV>::kThreads, 1) tree_t
     extern __shared__ __align__(1024) unsigned char tc_smem[];
     unsigned char* const smem = tc_smem;
     TcMisc& sm = *reinterpret_cast<TcMisc*>(smem + S::kMiscAt);
-    TcScales& sc = *reinterpret_cast<TcScales*>(smem + S::kMiscAt + sizeof(TcMisc));
-    static_assert(sizeof(TcMisc) % 16 == 0 && S::kMiscAt % 16 == 0, "vector reads of the scales behind");
-    static_assert((TILES == 2 ? offsetof(TcMisc, row) : sizeof(TcMisc)) + (KV == kTreeF16 ? 0 : sizeof(TcScales)) <= S::kMisc, "misc area");
+    // what lies behind `row` (TILES = 2) or `v_exp` (fp16 pages) is not there
+    constexpr uint32_t kMiscUsed = TILES == 2 ? offsetof(TcMisc, row) : KV == kTreeF16 ? offsetof(TcMisc, v_exp) : sizeof(TcMisc);
+    static_assert(kMiscUsed % 16 == 0 && kMiscUsed + (KV == kTreeF16 ? 0 : sizeof(TcScales)) <= S::kMisc, "misc area");
+    static_assert(S::kMiscAt % 16 == 0, "vector reads of the scales");
+    TcScales& sc = *reinterpret_cast<TcScales*>(smem + S::kMiscAt + kMiscUsed);
     const int tid = threadIdx.x, warp = tid >> 5, lane = tid & 31;
     const TcGiveUp give_up = {&sm.abort, pp.wait_cycles};
 
@@ -901,6 +904,28 @@ __global__ void __launch_bounds__(TcShape<D, TILES, QS, KV>::kThreads, 1) tree_t
                     tmem_wait_st();
                     ks = sc.one;
                 }
+                // ---- the step's unit: the largest V scale, where drafted tokens are among them the largest that the row
+                //      sees (a larger one beside it would push its weights below fp16), looked up if it can matter ----
+                int ex = -100;
+                bool own_unit = false;
+                if (KV != kTreeF16) {
+                    ex = sc.v_exp[e4];
+                    own_unit = masked && __any_sync(0xffffffffu, ex > v_exp);
+                    if (own_unit) {
+                        float v_top = 0.f;
+#pragma unroll 1
+                        for (int c = 0; c < 16 * NC; c += 16) {
+                            const uint32_t see = in ? tc_sees32(p, seg.row0, ti, seg.drafted, t0 + c - seg.ctx) : 0u;
+#pragma unroll
+                            for (int x = 0; x < 16; x += 4) {
+                                const float4 k = *reinterpret_cast<const float4*>(&sc.v[e4][col0 + c + x]);
+                                v_top = fmaxf(v_top, fmaxf(fmaxf((see >> x) & 1u ? k.x : 0.f, (see >> (x + 1)) & 1u ? k.y : 0.f),
+                                                           fmaxf((see >> (x + 2)) & 1u ? k.z : 0.f, (see >> (x + 3)) & 1u ? k.w : 0.f)));
+                            }
+                        }
+                        ex = max((int)(__float_as_uint(v_top) >> 23) - 126, -100);
+                    }
+                }
                 // ---- maximum ----
                 float tops[2] = {-INFINITY, -INFINITY};
                 tc_sweep<NC, false>(s_addr, [&](int c, float (&v)[16]) {
@@ -912,19 +937,20 @@ __global__ void __launch_bounds__(TcShape<D, TILES, QS, KV>::kThreads, 1) tree_t
                 if (TILES == 1) {
                     // behind this wait the other group has read its part of the O buffer, too
                     sm.row[i & 1][w][row] = top;
+                    if (KV != kTreeF16 && own_unit) sm.v_exp[i & 1][w][row] = ex;
                     tc_fence_before();
                     mbar_arrive(&sm.pair);
                     if (!tc_wait(&sm.pair, pair_phase, give_up)) { ok = false; break; }
                     pair_phase ^= 1u;
                     tc_fence_after();
                     top = fmaxf(top, sm.row[i & 1][w ^ 1][row]);
+                    if (KV != kTreeF16 && own_unit) ex = max(ex, sm.v_exp[i & 1][w ^ 1][row]);
                 }
                 const float m_new = top == -INFINITY ? m : fmaxf(m, top * mul);
                 const float f = tree_ex2(m - m_new);
                 float fo = f;                // O is kept in units of 2^v_exp, l is not
                 m = m_new;
                 if (KV != kTreeF16) {
-                    const int ex = sc.v_exp[e4];
                     if (ex > v_exp) {
                         fo *= ldexpf(1.0f, max(v_exp - ex, -126));
                         v_exp = ex;
