@@ -164,3 +164,15 @@ def test_large_v_scales_that_are_not_seen_do_not_reach_a_row(kernel, kv, name, p
         assert torch.equal(got[rest], clean[rest])
         if name == "f32":                    # fp16 results end at 65504
             case.check(got)
+
+
+@pytest.mark.parametrize("kernel", KERNELS)
+@pytest.mark.parametrize("kv", ["f16", "int8"])
+@pytest.mark.parametrize("name", ["f32", "bf16"])
+@pytest.mark.parametrize("power", [110, 120, -110])
+def test_queries_at_the_ends_of_their_range(kernel, kv, name, power):
+    """Queries of 2^power: with a scale to match the scores are ordinary ones."""
+    case = _case(kernel, [90, 40], [6, 8], kv, name, 107)
+    case.q = (case.q.double() * 2.0 ** power).to(case.q.dtype)
+    case.scale *= 2.0 ** -power
+    case.check(case.run())

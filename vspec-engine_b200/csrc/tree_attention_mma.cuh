@@ -161,7 +161,7 @@ __global__ void __launch_bounds__(kTreeThreads) tree_mma_kernel(const TreeParams
                 top = warp_max(top);
                 int ex = 14;
                 if (top > 0.f && top <= 3.402823466e+38f) (void)frexpf(top, &ex);
-                ex = max(-100, min(100, ex - 14));
+                ex = max(-126, ex - 14);             // at most 114
                 mul = ldexpf(1.0f, ex);
                 const float inv = ldexpf(1.0f, -ex);
 #pragma unroll

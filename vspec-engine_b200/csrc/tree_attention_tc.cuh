@@ -780,7 +780,7 @@ __global__ void __launch_bounds__(TcShape<D, TILES, QS, KV>::kThreads, 1) tree_t
                             for (int o = 4; o > 0; o >>= 1) top = fmaxf(top, __shfl_xor_sync(0xffffffffu, top, o));
                             // 2^ex with the row's largest value in [2^13, 2^14), as far as normal numbers reach
                             int ex = (int)(__float_as_uint(top) >> 23) - 126 - 14;
-                            ex = top > 0.f && top <= 3.402823466e+38f ? max(-100, min(100, ex)) : 0;
+                            ex = top > 0.f && top <= 3.402823466e+38f ? max(-126, ex) : 0;   // at most 114
                             mul = __uint_as_float((uint32_t)(127 + ex) << 23);
                             const float inv = __uint_as_float((uint32_t)(127 - ex) << 23);
 #pragma unroll
