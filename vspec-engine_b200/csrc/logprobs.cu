@@ -206,7 +206,7 @@ __global__ void __launch_bounds__(kLpThreads, 4) logprobs_kernel(const LpParams 
         __syncthreads();
     }
 
-    const float c = p.inv_t * 1.4426950408889634f;
+    const float c = fminf(p.inv_t * 1.4426950408889634f, -kLpLowest);   // finite, so that 0 * c is 0
     LpStats st = {kLpLowest, 0.f, 0.f};
     unsigned long long best = 0;   // the warp's best, in order over its lanes
     const int j_lane = (p.top_k + kLpWarps - 1) / kLpWarps - 1;
