@@ -319,7 +319,8 @@ int vspec_b200_paged_gather(const void* d_k_pages, const void* d_v_pages, const 
  * angles are held in 32 bits, results are rounded once.  Attention multiplies
  * fp32 queries and softmax weights as two fp16 parts, 22 bits.  Calls that
  * share a workspace, the library's for a device and host thread among them,
- * must be stream-ordered; a workspace's contents do not matter.
+ * must be stream-ordered; a workspace's contents do not matter.  Addresses are
+ * multiples of their values' size (ERR_ARG otherwise).
  * ------------------------------------------------------------------------ */
 #define VSPEC_B200_T_F32 0
 #define VSPEC_B200_T_F16 1

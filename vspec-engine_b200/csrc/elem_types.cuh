@@ -4,6 +4,8 @@
 
 #include "common.cuh"
 
+#include <initializer_list>
+
 namespace vb200 {
 
 template <typename T> __device__ __forceinline__ float elem_to_f32(T v);
@@ -33,7 +35,14 @@ inline int elem_vec(uintptr_t addresses, size_t counts) {
 }
 
 inline bool elem_type_known(int t) { return t == VSPEC_B200_T_F32 || t == VSPEC_B200_T_F16 || t == VSPEC_B200_T_BF16; }
+inline size_t elem_bytes(int t) { return t == VSPEC_B200_T_F32 ? 4 : 2; }
 
+// Whether one of the addresses is no multiple of its values' size, which would fault on the device.
+inline bool off_type(size_t size, std::initializer_list<const void*> addresses) {
+    for (const void* a : addresses)
+        if ((uintptr_t)a % size != 0) return true;
+    return false;
+}
 
 // Two fp32 values an instruction, each rounded as by itself.
 typedef unsigned long long pair32;

@@ -303,6 +303,9 @@ extern "C" int vspec_b200_kv_quant_append(const VspecB200KvQuantArgs* a, void* s
     if (!elem_type_known(a->src_dtype)) { set_error("bad src_dtype %d", a->src_dtype); return VSPEC_B200_ERR_ARG; }
     if (a->kv_dtype != VSPEC_B200_KV_FP8 && a->kv_dtype != VSPEC_B200_KV_INT8) { set_error("kv_dtype must be KV_FP8 or KV_INT8"); return VSPEC_B200_ERR_ARG; }
     if (!a->d_k || !a->d_v || !a->d_k_codes || !a->d_v_codes || !a->d_k_scales || !a->d_v_scales) { set_error("NULL pointer argument"); return VSPEC_B200_ERR_ARG; }
+    if (off_type(elem_bytes(a->src_dtype), {a->d_k, a->d_v}) || off_type(4, {a->d_slots, a->d_k_scales, a->d_v_scales})) {
+        set_error("rows, slots and scales must be aligned to their types"); return VSPEC_B200_ERR_ARG;
+    }
     if (a->num_kv_heads == 0 || a->head_dim == 0 || a->pool_rows == 0) { set_error("zero dimension"); return VSPEC_B200_ERR_ARG; }
     if (a->head_dim > kQuantMaxDim) { set_error("head_dim %zu is above %d", a->head_dim, kQuantMaxDim); return VSPEC_B200_ERR_UNSUPPORTED; }
     if (a->num_kv_heads > 8192 || a->rows > 0x7ffffff0u / a->num_kv_heads) { set_error("too many rows"); return VSPEC_B200_ERR_ARG; }
@@ -345,6 +348,10 @@ extern "C" int vspec_b200_kv_quant_gather(const VspecB200KvGatherArgs* a, void* 
     if (!a->d_k_codes || !a->d_v_codes || !a->d_k_scales || !a->d_v_scales || !a->d_page_table || !a->d_cu_tokens ||
         !a->d_k_out || !a->d_v_out) {
         set_error("NULL pointer argument"); return VSPEC_B200_ERR_ARG;
+    }
+    if (off_type(elem_bytes(a->out_dtype), {a->d_k_out, a->d_v_out}) ||
+        off_type(4, {a->d_k_scales, a->d_v_scales, a->d_page_table, a->d_cu_tokens})) {
+        set_error("scales, table, d_cu_tokens and outputs must be aligned to their types"); return VSPEC_B200_ERR_ARG;
     }
     if (a->batch == 0 || a->num_kv_heads == 0 || a->head_dim == 0 || a->page_tokens == 0 ||
         a->max_pages_per_seq == 0 || a->num_pages == 0) {

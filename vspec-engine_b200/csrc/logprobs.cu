@@ -492,8 +492,11 @@ extern "C" int vspec_b200_logprobs(const VspecB200LogprobsArgs* a, void* stream)
     if (!(a->inv_temperature >= 1e-30f) || isinf(a->inv_temperature)) { set_error("inv_temperature must be finite and at least 1e-30"); return VSPEC_B200_ERR_ARG; }
     if (!a->num_tokens && !a->d_entropy && !a->top_k) { set_error("no output is asked for"); return VSPEC_B200_ERR_ARG; }
     if (a->rows > 65535) { set_error("at most 65535 rows a call"); return VSPEC_B200_ERR_UNSUPPORTED; }
-    const size_t elem = a->dtype == VSPEC_B200_T_F32 ? 4 : 2;
-    if ((uintptr_t)a->d_logits % elem != 0) { set_error("logits are not aligned to their type"); return VSPEC_B200_ERR_ARG; }
+    if (off_type(elem_bytes(a->dtype), {a->d_logits})) { set_error("logits are not aligned to their type"); return VSPEC_B200_ERR_ARG; }
+    if (off_type(4, {a->d_allowed, a->d_tokens, a->d_token_logprobs, a->d_entropy, a->d_top_logprobs, a->d_top_ids})) {
+        set_error("tokens, allowed bits and results must be aligned to 4 bytes");
+        return VSPEC_B200_ERR_ARG;
+    }
     if (a->rows == 0) return VSPEC_B200_OK;
     LpParams p;
     memset(&p, 0, sizeof(p));

@@ -169,6 +169,10 @@ extern "C" int vspec_b200_rope(const VspecB200RopeArgs* a, void* stream) {
     if (a->flags & ~(VSPEC_B200_ROPE_INTERLEAVED | VSPEC_B200_ROPE_INVERSE)) { set_error("unknown rope flags 0x%x", a->flags); return VSPEC_B200_ERR_ARG; }
     if (!a->d_q || !a->d_q_out || !a->d_pos || !a->d_turns) { set_error("NULL pointer argument"); return VSPEC_B200_ERR_ARG; }
     if ((a->d_k == nullptr) != (a->d_k_out == nullptr)) { set_error("d_k and d_k_out go together"); return VSPEC_B200_ERR_ARG; }
+    if (off_type(elem_bytes(a->dtype), {a->d_q, a->d_k, a->d_q_out, a->d_k_out}) || off_type(4, {a->d_pos}) || off_type(8, {a->d_turns})) {
+        set_error("q, k, outputs, d_pos and d_turns must be aligned to their types");
+        return VSPEC_B200_ERR_ARG;
+    }
     const size_t hk = a->d_k ? a->num_k_heads : 0;
     if (a->num_q_heads == 0 || a->head_dim == 0 || (a->d_k && hk == 0)) { set_error("zero dimension"); return VSPEC_B200_ERR_ARG; }
     if (a->rot_dim == 0 || a->rot_dim % 2 != 0 || a->rot_dim > a->head_dim || a->head_dim > 512 || a->head_dim % 2 != 0) {

@@ -255,6 +255,7 @@ extern "C" int vspec_b200_tree_attention(const VspecB200TreeAttnArgs* a, void* s
     const uintptr_t al = (uintptr_t)a->d_q | (uintptr_t)a->d_k_pages | (uintptr_t)a->d_v_pages | (uintptr_t)a->d_out |
                          (f16 ? 0 : (uintptr_t)a->d_k_scales | (uintptr_t)a->d_v_scales);
     if (al % 16 != 0) { set_error("q, out, pages and scales must be 16-byte aligned"); return VSPEC_B200_ERR_ARG; }
+    if (off_type(4, {a->d_page_table, a->d_ctx_len, a->d_cu_q, a->d_mask})) { set_error("table, d_ctx_len, d_cu_q and d_mask must be aligned to 4 bytes"); return VSPEC_B200_ERR_ARG; }
     if (a->total_q == 0) return VSPEC_B200_OK;
 
     const TreePlan plan = tree_plan(a->batch, a->max_q, a->num_q_heads, a->num_kv_heads, a->head_dim, a->page_tokens, max_ctx, f16);
