@@ -446,7 +446,8 @@ typedef struct VspecB200TreeAttnArgs {
     float scale;
     int q_dtype;                  /* VSPEC_B200_T_* */
     int kv_dtype;                 /* VSPEC_B200_KV_F16, _FP8 or _INT8 */
-    void* d_workspace;            /* NULL = library-managed device scratch, grown on first use of a shape */
+    void* d_workspace;            /* NULL = library-managed device scratch of the host thread, grown on first
+                                     use of a shape (not inside a capture), given back when the thread ends */
     size_t workspace_bytes;
 } VspecB200TreeAttnArgs;
 size_t vspec_b200_tree_attention_workspace_bytes(size_t batch, size_t total_q, size_t max_q, size_t num_q_heads,
@@ -479,7 +480,8 @@ typedef struct VspecB200LogprobsArgs {
     size_t num_tokens, top_k;
     float inv_temperature;        /* at least 1e-30 */
     int dtype;                    /* VSPEC_B200_T_* */
-    void* d_workspace;            /* NULL = library-managed device scratch, grown on first use of a shape */
+    void* d_workspace;            /* NULL = library-managed device scratch of the host thread, grown on first
+                                     use of a shape (not inside a capture), given back when the thread ends */
     size_t workspace_bytes;
 } VspecB200LogprobsArgs;
 size_t vspec_b200_logprobs_workspace_bytes(size_t rows, size_t vocab, size_t top_k);

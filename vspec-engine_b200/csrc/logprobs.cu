@@ -15,6 +15,7 @@
 // have 4 and some 3); 8 rows, top 5, 14.4 us, most of it the chain of the first
 // block's selection, the parts' way to the last CTA and its join.
 #include "elem_types.cuh"
+#include "thread_scratch.cuh"
 
 #include <math.h>
 #include <string.h>
@@ -435,28 +436,8 @@ static size_t lp_workspace(size_t rows, size_t vocab, size_t top_k) {
     return s > 1 ? kLpCounterBytes + rows * s * (4 * sizeof(float) + top_k * sizeof(unsigned long long)) : 0;
 }
 
-// Library-managed scratch, one grow-only buffer per device and host thread;
-// its counters are zero between calls.
-struct LpScratch {
-    void* ptr;
-    size_t cap;
-};
-static thread_local LpScratch g_lp_scratch[64];
-
-static void* lp_scratch(size_t bytes, cudaStream_t st) {
-    int dev = 0;
-    if (cudaGetDevice(&dev) != cudaSuccess || dev < 0 || dev >= 64) return nullptr;
-    LpScratch& s = g_lp_scratch[dev];
-    if (s.cap < bytes) {
-        if (s.ptr) cudaFree(s.ptr);
-        s.ptr = nullptr;
-        s.cap = 0;
-        if (cudaMalloc(&s.ptr, bytes) != cudaSuccess) { s.ptr = nullptr; return nullptr; }
-        if (cudaMemsetAsync(s.ptr, 0, kLpCounterBytes, st) != cudaSuccess) { cudaFree(s.ptr); s.ptr = nullptr; return nullptr; }
-        s.cap = bytes;
-    }
-    return s.ptr;
-}
+// The counters in front of it are zero between calls.
+static thread_local ThreadScratch g_lp_scratch;
 
 template <typename T>
 static cudaError_t lp_launch(const LpParams& p, size_t rows, cudaStream_t st) {
@@ -526,8 +507,8 @@ extern "C" int vspec_b200_logprobs(const VspecB200LogprobsArgs* a, void* stream)
             // whatever used it before
             VB_CHECK_CUDA(cudaMemsetAsync(ws, 0, a->rows * sizeof(unsigned), st));
         } else {
-            ws = lp_scratch(need, st);
-            if (!ws) { set_error("cannot allocate %zu bytes of scratch", need); return VSPEC_B200_ERR_NOMEM; }
+            const int rc = g_lp_scratch.get(need, kLpCounterBytes, st, &ws);
+            if (rc != VSPEC_B200_OK) return rc;
         }
         p.counters = (unsigned*)ws;
         p.part_keys = (unsigned long long*)((char*)ws + kLpCounterBytes);

@@ -1,6 +1,7 @@
 // tree_attention.cu -- entry point of the tree attention: argument checks, the
 // plan (rows and context of a CTA) and the kernel that joins context pieces.
 #include "attention_kernels.cuh"
+#include "thread_scratch.cuh"
 #include "tree_attention_tc.cuh"
 
 #include <limits.h>
@@ -168,26 +169,7 @@ static size_t tree_parts(const TreePlan& t, size_t total_q, size_t max_q, size_t
 
 static std::atomic<long long> g_tree_wait_cycles{kTcWaitCycles};
 
-// Library-managed scratch, one grow-only buffer per device and host thread.
-struct TreeScratch {
-    void* ptr;
-    size_t cap;
-};
-static thread_local TreeScratch g_tree_scratch[64];
-
-static void* tree_scratch(size_t bytes) {
-    int dev = 0;
-    if (cudaGetDevice(&dev) != cudaSuccess || dev < 0 || dev >= 64) return nullptr;
-    TreeScratch& s = g_tree_scratch[dev];
-    if (s.cap < bytes) {
-        if (s.ptr) cudaFree(s.ptr);
-        s.ptr = nullptr;
-        s.cap = 0;
-        if (cudaMalloc(&s.ptr, bytes) != cudaSuccess) { s.ptr = nullptr; return nullptr; }
-        s.cap = bytes;
-    }
-    return s.ptr;
-}
+static thread_local ThreadScratch g_tree_scratch;
 
 }  // namespace vb200
 
@@ -289,8 +271,8 @@ extern "C" int vspec_b200_tree_attention(const VspecB200TreeAttnArgs* a, void* s
             if (a->workspace_bytes < need) { set_error("workspace too small (%zu < %zu)", a->workspace_bytes, need); return VSPEC_B200_ERR_ARG; }
             if ((uintptr_t)ws % 16 != 0) { set_error("workspace must be 16-byte aligned"); return VSPEC_B200_ERR_ARG; }
         } else {
-            ws = tree_scratch(need);
-            if (!ws) { set_error("cannot allocate %zu bytes of scratch", need); return VSPEC_B200_ERR_NOMEM; }
+            const int rc = g_tree_scratch.get(need, 0, (cudaStream_t)stream, &ws);
+            if (rc != VSPEC_B200_OK) return rc;
         }
         p.part_o = (float*)ws;
         p.part_ml = p.part_o + parts * a->head_dim;
