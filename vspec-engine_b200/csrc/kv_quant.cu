@@ -138,10 +138,12 @@ __global__ void __launch_bounds__(kQuantThreads) kv_quant_append_kernel(const Qu
             top[side] = m;
         }
     }
-    // the four quotients M / top and top / M of K and V, one a lane (LL >= 2)
+    // the four quotients M / top and top / M of K and V, one a lane (LL >= 2); where M / top would leave fp32, values
+    // and top are taken times 2^100
     constexpr float M = FP8 ? 448.0f : 127.0f;
+    constexpr float kTiny = 1e-35f, kUp = 1.2676506002282294e30f;
     const float mine = __uint_as_float((l & 1) ? top[1] : top[0]);
-    const float quot = __fdiv_rn((l & 2) ? mine : M, (l & 2) ? M : mine);
+    const float quot = __fdiv_rn((l & 2) ? mine : M, (l & 2) ? M : (mine > kTiny ? mine : mine * kUp));
     const float inv[2] = {__shfl_sync(0xffffffffu, quot, 0, lanes), __shfl_sync(0xffffffffu, quot, 1, lanes)};
     if (!inside || slot < 0) return;
     if ((size_t)slot >= p.pool_rows) {
@@ -153,8 +155,8 @@ __global__ void __launch_bounds__(kQuantThreads) kv_quant_append_kernel(const Qu
 #pragma unroll
     for (int side = 0; side < 2; ++side) {
         uint8_t* dst = (side ? p.v_codes : p.k_codes) + out_row * p.d;
-        // above 1e-35 inv stays finite
-        const bool fast = V % 4 == 0 && !odd[side] && __uint_as_float(top[side]) > 1e-35f;
+        const bool tiny = __uint_as_float(top[side]) <= kTiny;
+        const bool fast = V % 4 == 0 && !odd[side] && !tiny;
 #pragma unroll
         for (int c = 0; c < C; ++c) {
             const int at = (c * lanes + l) * V;
@@ -167,7 +169,7 @@ __global__ void __launch_bounds__(kQuantThreads) kv_quant_append_kernel(const Qu
                     if constexpr (V % 4 == 0) quant_fast<FP8, V>(v, inv[side], w);
                 } else {
 #pragma unroll
-                    for (int j = 0; j < V; ++j) w.e[j] = quant_code<FP8>(v[j], inv[side]);
+                    for (int j = 0; j < V; ++j) w.e[j] = quant_code<FP8>(tiny ? v[j] * kUp : v[j], inv[side]);
                 }
                 *reinterpret_cast<Vec<uint8_t, V>*>(dst + at) = w;
             }
