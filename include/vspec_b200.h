@@ -391,8 +391,9 @@ typedef struct VspecB200KvQuantArgs {
     int kv_dtype;                 /* VSPEC_B200_KV_FP8 or _INT8 */
 } VspecB200KvQuantArgs;
 /* Writes rows into the pools.  A slot at or past pool_rows is skipped and
- * reported by vspec_b200_paged_attention_page_fault(); two rows with one slot
- * leave either.  head_dim <= 512. */
+ * reported by vspec_b200_paged_attention_page_fault().  Slots of a call are
+ * distinct (but for skipped ones): rows that share one leave a mix of their
+ * codes and scales.  head_dim <= 512. */
 int vspec_b200_kv_quant_append(const VspecB200KvQuantArgs* args, void* stream);
 
 typedef struct VspecB200KvGatherArgs {
