@@ -1,5 +1,8 @@
 """Tree attention at the ends of its inputs' ranges, in the kernel for few rows
-and in the one for many."""
+and in the one for many, and what else the two have to share: streams, host
+threads, graphs, offsets, heads."""
+import threading
+
 import numpy as np
 import pytest
 
@@ -176,3 +179,116 @@ def test_queries_at_the_ends_of_their_range(kernel, kv, name, power):
     case.q = (case.q.double() * 2.0 ** power).to(case.q.dtype)
     case.scale *= 2.0 ** -power
     case.check(case.run())
+
+
+@pytest.mark.parametrize("kernel", KERNELS)
+@pytest.mark.parametrize("kv", ["fp8", "int8"])
+@pytest.mark.parametrize("order", ["up", "down"])
+def test_uneven_v_scales(kernel, kv, order):
+    """V scales over thirty orders of magnitude along the context."""
+    torch = torch_cuda()
+    case = _case(kernel, [640, 900], [8, 5], kv, "f32", 112)
+    for b, (c, n) in enumerate(zip(case.ctx, case.trees)):
+        scales = torch.logspace(-20, 10, c + n, device="cuda").unsqueeze(-1)
+        case.scales[1][_slots(case, b, np.arange(c + n))] = scales if order == "up" else scales.flip(0)
+    case.check(case.run())
+
+
+@pytest.mark.parametrize("kernel", KERNELS)
+@pytest.mark.parametrize("kv", ["f16", "fp8"])
+def test_graph_replays_follow_lengths(kernel, kv):
+    torch = torch_cuda()
+    case = _case(kernel, [500, 40], [6, 8], kv, "f16", 113)
+    need = V.lib.vspec_b200_tree_attention_workspace_bytes(2, case.total, 8, 8, 2, 128, case.max_ctx)
+    ws = torch.empty(max(need, 16), dtype=torch.uint8, device="cuda")
+    out = case.run(workspace=ws)
+    torch.cuda.synchronize()
+    table, ctx, cu, mask = case._keep
+    scales = [s.data_ptr() if s is not None else None for s in case.scales]
+    g = torch.cuda.CUDAGraph()
+    with torch.cuda.graph(g):
+        V.tree_attention(case.q.data_ptr(), case.codes[0].data_ptr(), case.codes[1].data_ptr(), *scales,
+                         table.data_ptr(), ctx.data_ptr(), cu.data_ptr(), mask.data_ptr(), out.data_ptr(), 2, case.total,
+                         8, 8, 2, 128, 16, case.table.shape[1], case.pages, case.max_ctx, case.scale, q_dtype=V.T_F16,
+                         kv_dtype=V.KV_F16 if kv == "f16" else V.KV_FP8, mask_words=case.words,
+                         workspace=ws.data_ptr(), workspace_bytes=ws.numel(),
+                         stream=torch.cuda.current_stream().cuda_stream)
+    for ctx_now, trees_now in (([500, 40], [6, 8]), ([7, 41], [8, 4]), ([300, 0], [6, 8]), ([127, 128], [1, 2])):
+        case.ctx, case.trees = ctx_now, trees_now
+        ctx.copy_(torch.tensor(ctx_now, dtype=torch.int32))
+        cu.copy_(torch.tensor([0] + list(np.cumsum(trees_now)), dtype=torch.int32))
+        g.replay()
+        out[sum(trees_now):] = 0
+        total, case.total = case.total, sum(trees_now)
+        q, case.q = case.q, case.q[:case.total]
+        case.check(out[:case.total])
+        case.total, case.q = total, q
+
+
+@pytest.mark.parametrize("kernel", KERNELS)
+def test_streams_and_host_threads(kernel):
+    """Two host threads, each on a stream of its own with the library's scratch, time and again."""
+    torch = torch_cuda()
+    cases = [_case(kernel, [900, 350], [8, 5], "f16", "f32", 114), _case(kernel, [300, 800], [6, 7], "fp8", "f32", 115)]
+    expect = [c.run().clone() for c in cases]
+    torch.cuda.synchronize()
+    got, wrong = [None, None], []
+
+    def work(i):
+        try:
+            st = torch.cuda.Stream()
+            with torch.cuda.stream(st):
+                for _ in range(20):
+                    got[i] = cases[i].run(stream=st.cuda_stream)
+                    st.synchronize()
+                    if not torch.equal(got[i], expect[i]):
+                        wrong.append(i)
+        except Exception as e:  # noqa: BLE001
+            wrong.append(e)
+
+    threads = [threading.Thread(target=work, args=(i,)) for i in range(2)]
+    for t in threads:
+        t.start()
+    for t in threads:
+        t.join()
+    assert not wrong
+    for c, out in zip(cases, expect):
+        c.check(out)
+
+
+@pytest.mark.parametrize("kv", ["f16", "int8"])
+def test_pool_offsets_past_32_bits_many_rows(kv):
+    """Pages beyond 2^31 elements of the pool."""
+    torch = torch_cuda()
+    case = _case("many rows", [100], [24], kv, "f32", 116, hq=8, hkv=8)
+    far = (1 << 31) // (16 * 8 * 128) + 5
+    rows = far * 16
+    pool = torch.empty((rows + case.codes[0].shape[0], 8, 128), dtype=case.codes[0].dtype, device="cuda")
+    pool[rows:] = case.codes[0]
+    case.codes = [pool, pool]
+    if kv != "f16":
+        wide = torch.empty((rows + case.scales[0].shape[0], 8), device="cuda")
+        wide[rows:] = case.scales[0]
+        case.scales = [wide, wide]
+    case.table = np.where(case.table >= 0, case.table + far, case.table).astype(np.int32)
+    case.pages += far
+    case.check(case.run())
+
+
+@pytest.mark.parametrize("kv", ["f16", "fp8", "int8"])
+@pytest.mark.parametrize("name", ["f32", "bf16"])
+@pytest.mark.parametrize("trees", [[4, 2], [9, 3], [20, 7]])
+def test_heads_of_256(kv, name, trees):
+    """One, two and four row warps."""
+    case = Case(torch_cuda(), np.random.default_rng(117), [333, 64], trees, 8, 4, 256, 16, kv, name)
+    case.check(case.run())
+
+
+@pytest.mark.parametrize("kernel", KERNELS)
+@pytest.mark.parametrize("kv", ["f16", "fp8", "int8"])
+def test_repeated_calls_are_identical(kernel, kv):
+    torch = torch_cuda()
+    case = _case(kernel, [1500, 1200], [8, 7], kv, "bf16", 118)
+    first = case.run().clone()
+    for _ in range(10):
+        assert torch.equal(case.run(), first)
