@@ -292,3 +292,19 @@ def test_repeated_calls_are_identical(kernel, kv):
     first = case.run().clone()
     for _ in range(10):
         assert torch.equal(case.run(), first)
+
+
+@pytest.mark.parametrize("kernel", KERNELS)
+@pytest.mark.parametrize("kv", ["f16", "int8"])
+@pytest.mark.parametrize("length", [1 << 20, (1 << 31) - 1])
+def test_lengths_past_the_page_table_are_told(kernel, kv, length):
+    """The flag is raised, and the other sequences are right."""
+    torch = torch_cuda()
+    case = _case(kernel, [500, 40], [6, 8], kv, "f32", 108)
+    ref, big = case.ref()
+    V.page_fault_flag()
+    case.ctx = [length, 40]
+    got = case.run()
+    torch.cuda.synchronize()
+    assert V.page_fault_flag() == 1 and V.tree_attention_timeout_flag() == 0
+    assert ((got.double() - ref).abs() / big)[6:].max().item() <= BOUND["f32"]

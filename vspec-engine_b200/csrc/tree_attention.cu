@@ -25,7 +25,7 @@ __global__ void __launch_bounds__(256) tree_combine_kernel(const TreeParams p) {
     const int lane = threadIdx.x & 31, w = WARPS > 1 ? (int)threadIdx.x >> 5 : 0;
     const long long r = WARPS > 1 ? (long long)blockIdx.x : (long long)blockIdx.x * 8 + (threadIdx.x >> 5);
     if (r >= (long long)drafted * p.hq) return;   // the same for all warps of a row
-    const int total = max(p.ctx_len[b], 0) + drafted;
+    const int total = tree_ctx(p, b) + drafted;
     const int n = tree_pieces(p, total);
     if (n <= 1) return;
     const size_t row = (size_t)row0 * p.hq + (size_t)r;
@@ -257,6 +257,8 @@ extern "C" int vspec_b200_tree_attention(const VspecB200TreeAttnArgs* a, void* s
     p.hq = (int)a->num_q_heads; p.hkv = (int)a->num_kv_heads; p.group = p.hq / p.hkv; p.d = (int)a->head_dim;
     p.page_tokens = (int)a->page_tokens; p.max_pages = (int)a->max_pages_per_seq; p.num_pages = (int)a->num_pages;
     p.mask_words = (int)a->mask_words;
+    const size_t most = lim - 4096 - a->max_q;
+    p.table_tokens = (int)(cap < most ? cap : most);
     p.split_tokens = plan.split_tokens; p.max_splits = plan.max_splits; p.row_tiles = plan.row_tiles;
     p.pair_cost = plan.pair_cost;
     p.q_type = a->q_dtype;

@@ -22,6 +22,7 @@ struct TreeParams {
     float scale;
     int batch, total_q, max_q, hq, hkv, group, d;
     int page_tokens, max_pages, num_pages, mask_words;
+    int table_tokens;   // of a sequence's row of the table, at most what keeps positions in 32 bits
     int split_tokens, max_splits, row_tiles;   // warp-MMA kernel
     int pair_cost;                             // tcgen05 kernel: steps' worth of time a pair takes besides its steps
     int q_type;
@@ -49,6 +50,10 @@ __device__ __forceinline__ int tree_rows(const TreeParams& p, int b, int& row0) 
     const int end = min(p.cu_q[b + 1], p.total_q);
     return row0 < 0 || row0 >= end ? 0 : min(end - row0, p.max_q);
 }
+
+// Committed tokens of sequence b.  A length past the page table is cut to it, which bounds positions and work whatever
+// the length is; the drafted tokens behind have no page then, and their lookups raise the fault flag.
+__device__ __forceinline__ int tree_ctx(const TreeParams& p, int b) { return min(max(p.ctx_len[b], 0), p.table_tokens); }
 
 // Context pieces of a sequence (warp-MMA kernel); the last takes what is left, also past the caller's max_ctx.
 __device__ __forceinline__ int tree_pieces(const TreeParams& p, int total) {

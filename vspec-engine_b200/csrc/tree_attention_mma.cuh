@@ -106,7 +106,7 @@ __global__ void __launch_bounds__(kTreeThreads) tree_mma_kernel(const TreeParams
     const int drafted = tree_rows(p, b, row0);
     const int rows = drafted * p.group;             // of this pair
     if (rt * MT >= rows) return;
-    const int ctx = max(p.ctx_len[b], 0);
+    const int ctx = tree_ctx(p, b);
     const int total = ctx + drafted;
     const int t_begin = split * p.split_tokens;
     if (t_begin >= total) return;                   // gridDim.x is max_splits

@@ -203,7 +203,7 @@ template <int RT>
 __device__ __forceinline__ long long tc_work(const TreeParams& p, int b, int& n, int& tiles) {
     int row0;
     const int drafted = tree_rows(p, b, row0);
-    const int total = max(p.ctx_len[b], 0) + drafted;
+    const int total = tree_ctx(p, b) + drafted;
     n = (total + kTcStep - 1) / kTcStep;
     tiles = (drafted * p.group + RT - 1) / RT;
     return drafted ? (long long)(n + p.pair_cost) * p.hkv * tiles : 0;
@@ -239,7 +239,7 @@ struct TcWalk {
             if (s.steps == 0) continue;        // only the pair's cost: the next CTA begins its first step
             s.b = b;
             s.drafted = tree_rows(p, b, s.row0);
-            s.ctx = max(p.ctx_len[b], 0);
+            s.ctx = tree_ctx(p, b);
             s.n = n;
             s.kvh = (int)pair / tiles;         // pairs of a sequence: at most 65535
             s.rt = (int)pair - s.kvh * tiles;
