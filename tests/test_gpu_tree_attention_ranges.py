@@ -308,3 +308,12 @@ def test_lengths_past_the_page_table_are_told(kernel, kv, length):
     torch.cuda.synchronize()
     assert V.page_fault_flag() == 1 and V.tree_attention_timeout_flag() == 0
     assert ((got.double() - ref).abs() / big)[6:].max().item() <= BOUND["f32"]
+
+
+@pytest.mark.parametrize("kv", ["f16", "fp8", "int8"])
+@pytest.mark.parametrize("name", ["f32", "f16", "bf16"])
+@pytest.mark.parametrize("d", [48, 64, 80, 128])
+def test_more_rows_than_a_tile(kv, name, d):
+    """129 to 280 rows a pair: one or two row tiles a CTA."""
+    case = Case(torch_cuda(), np.random.default_rng(119), [700, 0, 130], [33, 43, 70], 8, 2, d, 16, kv, name)
+    case.check(case.run())

@@ -126,9 +126,10 @@ static bool tree_uses_tc(long long rows, double tokens, size_t d, size_t page_to
 // What a change of pairs costs the tcgen05 kernel in its steps (q rows in, rows
 // out, an empty pipeline).  Sequences of 512..8192 tokens, 8 KV heads, us with 2 /
 // 3 / 4 / 6 / 8: 32 of 256 rows, fp32 q and fp16 pages 377 / 346 / 334 / 314 / 313,
-// fp16 q 267 / - / 241 / 226; 32 of 96 rows 196 / 185 / 179 / 179.  Steps on 8-bit
-// pages take longer: 16 of 256 rows - / 226 / 224 / 235, 8 of 64 rows (1024..6144
-// tokens) 59.1 / 57.8 / 61.2 / 60.7.
+// fp16 q (one part a weight then) 267 / - / 241 / 226; 32 of 96 rows 196 / 185 /
+// 179 / 179.  Steps on 8-bit pages take longer, fp16 q with 3 / 4: 32 of 256 rows
+// 430 / 417, 16 of 256 218 / 216, heads of 64 162 / 165; with 2 / 3 / 4 / 6 (one
+// part a weight) 8 of 64 rows (1024..6144 tokens) 59.1 / 57.8 / 61.2 / 60.7.
 static int tree_pair_cost(long long rows, bool f16) { return f16 ? (rows > 128 ? 6 : 4) : (rows > 128 ? 4 : 3); }
 
 // Warp-MMA: rows a CTA 16, 32 or 64, the fewest that hold a pair's rows; context

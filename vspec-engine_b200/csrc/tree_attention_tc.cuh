@@ -1188,20 +1188,22 @@ cudaError_t tree_tc_launch_one(const TcParams& pp, int ctas, cudaStream_t st) {
     return launch_pdl(tree_tc_combine_kernel<128 * TILES>, dim3(ctas - 1, 4 * TILES), dim3(256), 0, st, pp.t);
 }
 
-// Row tiles a CTA: two for pairs of more than 128 rows; 8-bit pages with fp32 q
-// have no room for the two tiles' parts beside the raw ring.
-inline int tree_tc_tiles(int rows, bool f16_pages, int q_type) {
-    return rows > 128 && (f16_pages || q_type != VSPEC_B200_T_F32) ? 2 : 1;
-}
+// Row tiles a CTA: two for pairs of more than 128 rows; over 8-bit pages only for
+// heads of at most 64 and 16-bit q.  Heads of 128 need 128 registers for a row's
+// output, which beside the widening warps' share spill (one tile / two, fp16 q,
+// fp8 pages of 512..8192 tokens, us: 16 x 256 rows 216 / 264, 4 x 132 rows 69 /
+// 91; heads of 64: 199 / 166, 64 / 62), and two tiles' two-part q has no room.
+constexpr bool tree_tc_two_tiles(int d, bool f16_pages, bool f32_q) { return f16_pages || (d <= 64 && !f32_q); }
 
 template <int D, int KV>
 cudaError_t tree_tc_pick(const TcParams& pp, int ctas, cudaStream_t st) {
-    const bool two = pp.t.q_type == VSPEC_B200_T_F32;
-    const int tiles = tree_tc_tiles(pp.t.max_q * pp.t.group, KV == kTreeF16, pp.t.q_type);
-    if (tiles == 1) return two ? tree_tc_launch_one<D, 1, 2, KV>(pp, ctas, st) : tree_tc_launch_one<D, 1, 1, KV>(pp, ctas, st);
-    if constexpr (KV == kTreeF16)
-        if (two) return tree_tc_launch_one<D, 2, 2, KV>(pp, ctas, st);
-    return tree_tc_launch_one<D, 2, 1, KV>(pp, ctas, st);
+    constexpr bool f16 = KV == kTreeF16;
+    const bool two = pp.t.q_type == VSPEC_B200_T_F32, many = pp.t.max_q * pp.t.group > 128;
+    if constexpr (tree_tc_two_tiles(D, f16, true))
+        if (many && two) return tree_tc_launch_one<D, 2, 2, KV>(pp, ctas, st);
+    if constexpr (tree_tc_two_tiles(D, f16, false))
+        if (many && !two) return tree_tc_launch_one<D, 2, 1, KV>(pp, ctas, st);
+    return two ? tree_tc_launch_one<D, 1, 2, KV>(pp, ctas, st) : tree_tc_launch_one<D, 1, 1, KV>(pp, ctas, st);
 }
 
 // Boxes of box_rows pool rows x one KV head x 64 fp16 values or a whole row of D codes.
