@@ -422,8 +422,8 @@ int vspec_b200_kv_quant_gather(const VspecB200KvGatherArgs* args, void* stream);
  *   out[i][h] = softmax_j(q[i][h] . K_j * scale) V_j,  kv head = h / (Hq/Hkv).
  * d_mask NULL: j <= i (a chain, or a chunk of a prompt).  A row that sees
  * nothing yields zeros; what a row does not see does not reach it, infinities
- * and NaN included.  Pages as in vspec_b200_paged_attention (fp16), or 8-bit
- * codes with scales as above.  max_q 1 is plain decode.  head_dim <= 256, a
+ * and NaN included.  Pages as in vspec_b200_paged_attention (fp16, filled by the
+ * caller), or 8-bit codes with scales as above.  max_q 1 is plain decode.  head_dim <= 256, a
  * multiple of 8 (fp16 pages) or 16 (8-bit); pages, scales, q and out 16-byte
  * aligned, q_stride a multiple of 8.
  */
@@ -434,7 +434,8 @@ typedef struct VspecB200TreeAttnArgs {
     const float* d_k_scales;      /* 8-bit pages only */
     const float* d_v_scales;
     const int32_t* d_page_table;  /* [batch][max_pages_per_seq] */
-    const int32_t* d_ctx_len;     /* [batch] committed tokens */
+    const int32_t* d_ctx_len;     /* [batch] committed tokens; what passes the page table is cut off and raises
+                                     the page fault flag */
     const int32_t* d_cu_q;        /* [batch + 1] first row of each sequence; NULL = b * max_q */
     const uint32_t* d_mask;       /* [total_q][mask_words], or NULL */
     void* d_out;                  /* [total_q][num_q_heads][head_dim], q_dtype */
@@ -451,6 +452,7 @@ typedef struct VspecB200TreeAttnArgs {
                                      use of a shape (not inside a capture), given back when the thread ends */
     size_t workspace_bytes;
 } VspecB200TreeAttnArgs;
+/* With max_ctx as the call will have it, or the page table's capacity for a call's 0. */
 size_t vspec_b200_tree_attention_workspace_bytes(size_t batch, size_t total_q, size_t max_q, size_t num_q_heads,
                                                  size_t num_kv_heads, size_t head_dim, size_t max_ctx);
 int vspec_b200_tree_attention(const VspecB200TreeAttnArgs* args, void* stream);

@@ -5,10 +5,11 @@
 //
 // one scale a row of head_dim values.  Both are memory-bound: a row is read
 // once, held in registers between the maximum and the rounding, and its codes
-// written once.  Measured, 8 heads of 128: 16384 rows of fp16 to int8 19.5 us,
-// 5.2 TB/s (80 % of a copy's rate; the SMs issue 81 % of the time), 512 rows 2.5
-// us in a graph; 16384 tokens of fp8 pages to fp16 19.3 us, 5.3 TB/s, 777 tokens
-// 4.1 us.
+// written once.  Measured, 8 heads of 128, replayed in a graph: 16384 rows of fp16
+// to int8 20.3 us, 5.0 TB/s (77 % of a copy's rate; the SMs issue 82 % of the
+// time), 512 rows of fp32 to fp8 2.4 us; 16384 tokens of fp8 pages to fp16 22.6
+// us, 4.5 TB/s (69 %: the SMs issue 46 % of the time, warps wait for a token's page
+// and then for its codes), 777 tokens 4.0 us.
 #include "elem_types.cuh"
 #include "attention_kernels.cuh"
 

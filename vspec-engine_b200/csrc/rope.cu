@@ -14,10 +14,11 @@
 // and token, kept in shared memory) while the first rows are on their way, then
 // every thread walks over the heads of each token with a fixed place in the
 // head.  Without the sharing, 16 threads with the same place computed the same
-// sines and those took longer than the rows (75 us).  Measured: 8192 tokens of 32
-// + 8 heads of 128 in bf16, half of the dims rotated, 36.4 us, 4.6 TB/s read and written
-// (26 us at the rate of a copy; a third of the warps' time is the angles, which
-// the first rows' loads only partly cover); 8 tokens 2.0 us in a graph.
+// sines and those took longer than the rows (75 us).  Measured in a graph: 8192
+// tokens of 32 + 8 heads of 128 in bf16, half of the dims rotated, 35.9 us, 4.7
+// TB/s read and written (26 us at the rate of a copy).  What is left is latency: 42
+// % of the warps are active and wait for their rows, and the angles, a third of a
+// warp's time, lie between its loads and stores.  8 tokens 1.9 us.
 #include "elem_types.cuh"
 
 #include <math.h>

@@ -108,14 +108,16 @@ struct TreePlan {
 // Which kernel: rows are a pair's at most, its drafted tokens times the group's
 // heads.  The warp-MMA kernel's time grows with a pair's 16-row tiles, the tcgen05
 // kernel's, whose tile is 128 rows, does not, but its first result comes later
-// (21 us a call with next to nothing to read, against 13 to 22).  So tcgen05 from
+// (22 us a call with next to nothing to read, against 13 to 20).  So tcgen05 from
 // 17 rows on if tiles * tokens of all pairs reach 2^18, and above 64 rows, where
 // the other kernel reads the cache more than once, always.  Warp-MMA / tcgen05, us,
-// f16 pages and queries, heads of 128, 8 KV heads:
-//   16 rows:  1 x 8192 tokens  22 /  43,  16 x 2048  56 /  55,  16 x 8192  139 / 149
-//   32 rows:  1 x 8192         28 /  43,   4 x 2048  28 /  29,  16 x 1024   49 /  39
-//   64 rows:  1 x 2048         23 /  27,   4 x  512  23 /  23,  16 x 2048  102 /  56
-//  128 rows:  1 x  256         22 /  21,   4 x 1024  42 /  26,  16 x 2048  154 /  57
+// f16 queries, heads of 128, 8 KV heads, f16 pages, fp8 pages:
+//   16 rows:  1 x 8192 tokens  25 /  41,  26 /  46,  16 x 2048  55 /  56,  65 /  71,  16 x 8192 122 / 154, 181 / 188
+//   32 rows:  1 x 8192         31 /  42,  33 /  47,   4 x 2048  30 /  30,  32 /  35,  16 x 1024  60 /  38,  63 /  52
+//   64 rows:  1 x 2048         19 /  26,  24 /  29,   4 x  512  21 /  22,  24 /  26,  16 x 2048 121 /  58, 144 /  72
+//  128 rows:  1 x  256         19 /  22,  20 /  22,   4 x 1024  49 /  26,  52 /  29,  16 x 2048 170 /  59, 218 /  74
+// fp32 queries move both sides by about a fifth (32 rows, 4 x 2048: 34 / 32).  Other
+// heads and numbers of KV heads go by the same rule; they were not timed.
 // Heads above 128 do not fit the tcgen05 kernel's registers (a row's output a
 // thread), pages of other than 8 k tokens its TMA boxes.
 static bool tree_uses_tc(long long rows, double tokens, size_t d, size_t page_tokens) {

@@ -19,8 +19,10 @@
 // scale over a running power of two), so that small weights stay normal.
 //
 // Bound by the latency of a short chain of loads when there is little to read:
-// 8 drafted tokens over 768, 4 heads a KV head, 10.4 us, 15 with the joining
-// kernel.  8 x 32768 tokens, 4 rows a pair: 238 us, 4.5 TB/s of fp16 pages.
+// 8 drafted tokens over 768, 4 heads a KV head, 15.3 us in a graph with the joining
+// kernel.  8 x 32768 tokens, 4 rows a pair: 203 us with fp16 q, 5.3 TB/s of fp16
+// pages, 258 us with fp32 q.  32 x 1 tokens over 2048..6144: 118 us of fp16 pages
+// (5.5 TB/s), 170 of fp8 (twice the steps a byte).
 #pragma once
 
 #include "tc_primitives.cuh"

@@ -24,15 +24,16 @@
 // the parts of such pairs in order.  fp32 q, weights and 8-bit pages are split
 // and scaled as in the warp-MMA kernels.
 //
-// Measured, 8 KV heads of 128, 16-token pages: 32 x 64 drafted tokens, 4 query
-// heads a KV head, contexts 512..8192, fp32 q and fp16 pages 312 us: 940
-// TFLOP/s of issued products (each of the two fp32 parts), 58 % of a cuBLAS
-// GEMM's rate.  A step takes 3.6 us, of which the products need 3.0; a change of
-// pairs (q rows, rows out, an empty pipeline) about 20 us, 2.7 of them a CTA.
-// 8 x 16 drafted tokens on fp8 pages, contexts 1024..6144: 57.5 us; 8 x 32768
-// tokens, 64 rows a pair: 4.1 TB/s of fp16 pages (262 us) and 1.6 TB/s of fp8
-// pages (336 us), bound by the latency of the softmax's steps and, for fp8, by
-// the instructions of the widening beside them (a stall in four is for code).
+// Measured, 8 KV heads of 128, 16-token pages, 4 query heads a KV head: 32 x 64
+// drafted tokens over 512..8192, fp32 q and fp16 pages, 310 us replayed in a graph,
+// 352 to 362 us a call with other inputs in between: 950 and 820 TFLOP/s of issued
+// products (two parts of q, two of the weights), 58 and 50 % of a cuBLAS GEMM's
+// rate; with fp16 q 260 us.  A step takes 3.6 us with fp32 q, of which the products
+// need 3.0; a change of pairs (q rows, rows out, an empty pipeline) about 20 us, 2.7
+// of them a CTA.  8 x 16 drafted tokens on fp8 pages, fp16 q, 1024..6144: 62 us.  8 x
+// 32768 tokens, 64 rows a pair, fp16 q: 3.8 TB/s of fp16 pages (279 us) and 1.6 TB/s
+// of fp8 pages (353 us), bound by the latency of the softmax's steps and, for
+// 8-bit pages, by the instructions of the widening beside them.
 #pragma once
 
 #include <stddef.h>
